@@ -37,6 +37,7 @@ STATUS_NAMES = {
 
 DTYPE_BF16 = 1
 DTYPE_FP8_E4M3FN = 2
+DTYPE_FP32 = 3
 
 FLAG_BF16_MFMA = 1
 FLAG_EXACT_EXP2 = 2
@@ -71,6 +72,12 @@ EXPORTED_SYMBOLS = (
     "pcpa_absmax_pair_bf16",
     "pcpa_block_mask_valid_len",
     "pcpa_page_alloc",
+    "pcpa_rotate",
+    "pcpa_chunk_write",
+    "pcpa_chunk_prepare",
+    "pcpa_cache_read",
+    "pcpa_chunk_workspace_bytes",
+    "pcpa_chunk_attention",
 )
 
 
@@ -94,6 +101,44 @@ class PcpaParams(ctypes.Structure):
         ("k_scale", ctypes.c_float),
         ("v_scale", ctypes.c_float),
         ("flags", ctypes.c_uint32),
+    ]
+
+
+class PcpaChunk(ctypes.Structure):
+    """Mirror of ``pcpa_chunk``."""
+
+    _fields_ = [
+        ("interleave", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("lengths", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+    ]
+
+
+class PcpaRows(ctypes.Structure):
+    """Mirror of ``pcpa_rows``."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
+class PcpaRotary(ctypes.Structure):
+    """Mirror of ``pcpa_rotary``."""
+
+    _fields_ = [
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("amplitude", ctypes.c_float),
+        ("norm_eps", ctypes.c_float),
+        ("turns", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
     ]
 
 
@@ -186,6 +231,21 @@ def load_library() -> ctypes.CDLL:
     lib.pcpa_page_alloc.restype = ctypes.c_int32
     lib.pcpa_page_alloc.argtypes = [ctypes.POINTER(PcpaParams), ctypes.c_int32, ctypes.c_int64, ctypes.c_int32,
                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    params, chunk, rows = ctypes.POINTER(PcpaParams), ctypes.POINTER(PcpaChunk), ctypes.POINTER(PcpaRows)
+    rotary, pointer = ctypes.POINTER(PcpaRotary), ctypes.c_void_p
+    lib.pcpa_rotate.restype = ctypes.c_int32
+    lib.pcpa_rotate.argtypes = [params, chunk, rotary, pointer, ctypes.c_int32, ctypes.c_int64] + [rows] * 6 + [
+        ctypes.c_int32, pointer]
+    lib.pcpa_chunk_write.restype = ctypes.c_int32
+    lib.pcpa_chunk_write.argtypes = [params, chunk, rows, rows] + [pointer] * 4
+    lib.pcpa_chunk_prepare.restype = ctypes.c_int32
+    lib.pcpa_chunk_prepare.argtypes = [params, chunk, rotary] + [rows] * 4 + [pointer] * 4
+    lib.pcpa_cache_read.restype = ctypes.c_int32
+    lib.pcpa_cache_read.argtypes = [params, ctypes.c_int32, ctypes.c_int64, ctypes.c_int32] + [pointer] * 6
+    lib.pcpa_chunk_workspace_bytes.restype = ctypes.c_int64
+    lib.pcpa_chunk_workspace_bytes.argtypes = [params, chunk]
+    lib.pcpa_chunk_attention.restype = ctypes.c_int32
+    lib.pcpa_chunk_attention.argtypes = [params, chunk] + [pointer] * 7 + [ctypes.c_int64, pointer]
     _lib = lib
     return lib
 

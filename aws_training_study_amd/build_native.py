@@ -1,9 +1,10 @@
 """Build the gfx950 HIP library in-tree with hipcc.
 
 ``python -m aws_training_study_amd.build_native`` compiles
-``csrc/pcp_attention_hip.hip`` (which includes the kernel headers in
-``csrc/``) into ``_lib/libpcp_attention_hip.so``.  hipcc cross-compiles for
-gfx950 without a GPU present.  Then g++ builds ``csrc/fast_calls.cpp``, the
+``csrc/pcp_attention_hip.hip`` (prefill and cache producer) and
+``csrc/serving.hip`` (chunks of new tokens over paged caches), which include
+the kernel headers in ``csrc/``, into ``_lib/libpcp_attention_hip.so``.  hipcc
+cross-compiles for gfx950 without a GPU present.  Then g++ builds ``csrc/fast_calls.cpp``, the
 Python entry points' per-call host path, into ``_lib/_pcpa_fast_calls.so`` and
 gcc ``csrc/abi_example.c``, a plain C caller of the library, into
 ``_lib/abi_example``.
@@ -20,6 +21,7 @@ from pathlib import Path
 PACKAGE_DIR = Path(__file__).resolve().parent
 REPO_ROOT = PACKAGE_DIR.parent
 SOURCES = [PACKAGE_DIR / "csrc" / "pcp_attention_hip.hip"]
+SERVING_SOURCES = [PACKAGE_DIR / "csrc" / "serving.hip"]
 INCLUDE_DIR = REPO_ROOT / "include"
 OUTPUT = PACKAGE_DIR / "_lib" / "libpcp_attention_hip.so"
 FAST_CALLS_SOURCE = PACKAGE_DIR / "csrc" / "fast_calls.cpp"
@@ -58,7 +60,7 @@ def compile_command(output: Path = OUTPUT) -> list[str]:
         "-fPIC",
         f"-I{INCLUDE_DIR}",
         *DEVICE_FLAGS,
-        *[os.fspath(s) for s in SOURCES],
+        *[os.fspath(s) for s in SOURCES + SERVING_SOURCES],
         "-o",
         os.fspath(output),
     ]

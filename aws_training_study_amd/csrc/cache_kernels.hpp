@@ -237,7 +237,7 @@ __device__ __forceinline__ int filled_slots(const FillArgs& a, int entry) {
 // 3 us here, 19 us to clear its 134 MB first); beyond kMaxScan (page, entry)
 // pairs the host asks for whole pages (scan 0).
 constexpr int64_t kMaxScan = 1ll << 24;
-__global__ void __launch_bounds__(kThreads) fill_rest_kernel(FillArgs a) {
+static __global__ void __launch_bounds__(kThreads) fill_rest_kernel(FillArgs a) {
     __shared__ int most[kThreads / 64];
     const int page = blockIdx.x, entries = a.pcp * a.max_local_blocks;
     const int64_t part = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, parts = (int64_t)gridDim.x * gridDim.y;
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads) fill_rest_kernel(FillArgs a) {
 
 // max |x| over n bf16 values into *out (as the bits of a non-negative float,
 // ordered like unsigned integers); *out is cleared first by init_kernel.
-__global__ void absmax_init_kernel(uint32_t* out) { out[threadIdx.x] = 0u; }
+static __global__ void absmax_init_kernel(uint32_t* out) { out[threadIdx.x] = 0u; }
 
 // |x| of the two bf16 values of a dword, as their 15-bit magnitude patterns.
 // Non-negative IEEE values order like their bit patterns, and every NaN
@@ -282,7 +282,7 @@ __device__ __forceinline__ uint32_t abs_bits_max(uint32_t m, uint32_t word) {
 // Workgroup b reduces the contiguous span [b * span, (b + 1) * span) with
 // four 16-byte loads in flight per thread, then one atomic per workgroup.
 // Grid y: x, or x and then `second` (of n values too, into out[1]).
-__global__ void __launch_bounds__(kThreads) absmax_kernel(const uint16_t* x, const uint16_t* second, int64_t n,
+static __global__ void __launch_bounds__(kThreads) absmax_kernel(const uint16_t* x, const uint16_t* second, int64_t n,
                                                           int64_t span, uint32_t* out) {
     if (blockIdx.y) {
         x = second;

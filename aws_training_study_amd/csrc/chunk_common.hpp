@@ -1,0 +1,93 @@
+// Chunks of new tokens over the striped paged caches of several sequences:
+// which sequence and position a row has, and where a position's page is.
+#pragma once
+
+#include "common.hpp"
+#include "paging_kernels.hpp"
+
+namespace pcpa {
+namespace chunk {
+
+struct Desc {
+    const int32_t* lengths;  // [batch]
+    const int32_t* starts;   // [batch + 1], or null: `each` rows per sequence
+    int32_t batch;
+    int32_t num_tokens;
+    int32_t each;
+};
+
+// The rows [first, first + count) of sequence b, within [0, num_tokens)
+// whatever `starts` holds.
+struct Span {
+    int32_t first;
+    int32_t count;
+};
+__device__ __forceinline__ Span span_of(const Desc& c, int b) {
+    if (!c.starts) return Span{b * c.each, c.each};
+    const int lo = min(max(c.starts[b], 0), c.num_tokens), hi = min(max(c.starts[b + 1], 0), c.num_tokens);
+    return Span{lo, max(hi - lo, 0)};
+}
+
+// The sequence of row `token` (wave-uniform), or -1 for a row of none; every
+// lane of the wave must be active.  The lanes count the sequences that end
+// before the row, 64 at a time: a binary search is six dependent loads for 64
+// sequences, this is one.
+__device__ __forceinline__ int sequence_of(const Desc& c, int token) {
+    if (!c.starts) return token / c.each;
+    const int lane = threadIdx.x & 63;
+    int b = 0;
+    for (int base = 0; base < c.batch; base += 64) {
+        const bool ended = base + lane < c.batch && c.starts[base + lane + 1] <= token;
+        b += __builtin_popcountll(__builtin_amdgcn_ballot_w64(ended));
+    }
+    if (b >= c.batch) return -1;
+    const Span s = span_of(c, b);
+    return token >= s.first && token < s.first + s.count ? b : -1;
+}
+
+struct Pages {
+    const int32_t* table;  // [batch, pcp, max_local_blocks], int32 or int64 as dword pairs
+    int32_t table_shift;
+    int32_t num_pages;
+    int32_t max_local_blocks;
+    int32_t block_size;
+    int32_t pcp;
+    int32_t interleave;
+    int32_t num_kv_heads;
+    int32_t capacity;      // positions of a sequence's cache: pcp * max_local_blocks * block_size
+    int64_t page_stride;   // bytes of a page
+    int64_t head_stride;   // bytes of one head's K (or V) of a page
+};
+
+// Entry `e` of a table whose first entry is `first` (64-bit: a batch of tables
+// may pass 2^31 entries), or -1 where it names no page.
+__device__ __forceinline__ int page_at(const Pages& p, int64_t first, int e) {
+    const int64_t i = (first + e) << p.table_shift;
+    const int page = p.table[i];
+    const bool good = (unsigned)page < (unsigned)p.num_pages && !(p.table_shift && p.table[i + 1] != 0);
+    return good ? page : -1;
+}
+__device__ __forceinline__ int64_t table_of(const Pages& p, int b) { return (int64_t)b * p.pcp * p.max_local_blocks; }
+
+// Page and slot of position `pos` (page -1: none) in the table at `first`.
+struct Place {
+    int page;
+    int slot;
+};
+__device__ __forceinline__ Place place_of(const Pages& p, int64_t first, int64_t pos) {
+    if (pos < 0 || pos >= p.capacity) return Place{-1, 0};
+    const uint32_t at = (uint32_t)pos, il = p.interleave, pcp = p.pcp;
+    const uint32_t c = at / il, round = c / pcp, rank = c - round * pcp;
+    const uint32_t local = round * il + (at - c * il);
+    const uint32_t blk = local / (uint32_t)p.block_size;
+    // (the last round of a bucket that is no whole number of rounds)
+    if (blk >= (uint32_t)p.max_local_blocks) return Place{-1, 0};
+    return Place{page_at(p, first, (int)(rank * p.max_local_blocks + blk)), (int)(local - blk * p.block_size)};
+}
+
+// The smallest scale of a row: quotients by it are exact to the rounding of
+// cache::div_rn, and a row of zeros needs no case of its own.
+constexpr float kScaleFloor = 0x1p-80f;
+
+}  // namespace chunk
+}  // namespace pcpa

@@ -17,7 +17,7 @@ constexpr int kAllocThreads = 1024;
 // consumed by kernel.py:113-118 and 341-358: 0 for a valid key, -9984 for
 // padding, always a prefix per block).  Every rank gets the same length
 // (the reference shares one mask among its ranks).
-__global__ void __launch_bounds__(kMaskThreads) mask_lengths_kernel(const uint16_t* mask, int block_size,
+static __global__ void __launch_bounds__(kMaskThreads) mask_lengths_kernel(const uint16_t* mask, int block_size,
                                                                     int max_local_blocks, int pcp,
                                                                     int32_t* page_valid_len) {
     __shared__ int wave_min[kMaskThreads / 64];
@@ -62,7 +62,7 @@ struct AllocArgs {
 // stack height is lowered by the pages taken.  Entries that find the stack
 // empty keep their negative value.  Deterministic: the same appends always
 // give the same table.
-__global__ void __launch_bounds__(kAllocThreads) page_alloc_kernel(AllocArgs a) {
+static __global__ void __launch_bounds__(kAllocThreads) page_alloc_kernel(AllocArgs a) {
     __shared__ int wave_count[kAllocThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int height = *a.free_count;

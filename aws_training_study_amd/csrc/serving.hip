@@ -1,0 +1,297 @@
+// C ABI of the serving operators (include/pcp_attention_hip.h): rows of new
+// tokens normed, rotated and written to the pages of their sequences
+// (token_kernels.hpp), a cache read back, and the causal attention of a chunk
+// over its sequences' caches (chunk_attention.hpp).
+#include "chunk_attention.hpp"
+#include "token_kernels.hpp"
+
+namespace pcpa {
+namespace chunk {
+namespace {
+
+// The parameters and the chunk, without the pointers that the kernels read.
+int32_t check_chunk(const pcpa_params* p, const pcpa_chunk* c) {
+    const int32_t st = pcpa_check_params(p);
+    if (st != PCPA_OK) return st;
+    if (!c) return PCPA_ERR_NULL_POINTER;
+    if (c->interleave <= 0 || c->batch <= 0 || c->num_tokens < 0 || c->reserved != 0) return PCPA_ERR_BAD_SHAPE;
+    if (!c->starts && c->num_tokens % c->batch) return PCPA_ERR_BAD_SHAPE;
+    if (((uintptr_t)c->lengths | (uintptr_t)c->starts) & 3u) return PCPA_ERR_MISALIGNED;
+    const int64_t capacity = (int64_t)p->pcp_size * p->max_local_blocks * p->block_size;
+    if (capacity > INT32_MAX || (int64_t)p->pcp_size * c->interleave > INT32_MAX ||
+        (int64_t)c->num_tokens * p->num_q_heads > INT32_MAX)
+        return PCPA_ERR_TOO_LARGE;
+    return PCPA_OK;
+}
+
+// The pages of a launch; the table holds `batch` sequences.
+int32_t check_pages(const pcpa_params* p, const void* block_table, const void* kv_pages, const float* token_scales) {
+    if (!block_table || !kv_pages) return PCPA_ERR_NULL_POINTER;
+    if ((uintptr_t)kv_pages & 15u) return PCPA_ERR_MISALIGNED;
+    if ((uintptr_t)block_table & ((p->flags & PCPA_FLAG_TABLE_INT64) ? 7u : 3u)) return PCPA_ERR_MISALIGNED;
+    if ((uintptr_t)token_scales & 15u) return PCPA_ERR_MISALIGNED;
+    if (token_scales && p->kv_dtype != PCPA_DTYPE_FP8_E4M3FN) return PCPA_ERR_BAD_DTYPE;
+    if (token_scales && (p->k_scale != 1.f || p->v_scale != 1.f)) return PCPA_ERR_BAD_SCALE;
+    return PCPA_OK;
+}
+
+Desc desc_of(const pcpa_chunk* c) {
+    return Desc{c->lengths, c->starts, c->batch, c->num_tokens, c->starts ? 0 : c->num_tokens / c->batch};
+}
+
+Pages pages_of(const pcpa_params* p, int32_t interleave, const void* block_table) {
+    const int64_t es = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN ? 1 : 2;
+    Pages g{};
+    g.table = (const int32_t*)block_table;
+    g.table_shift = (p->flags & PCPA_FLAG_TABLE_INT64) ? 1 : 0;
+    g.num_pages = p->num_pages;
+    g.max_local_blocks = p->max_local_blocks;
+    g.block_size = p->block_size;
+    g.pcp = p->pcp_size;
+    g.interleave = interleave;
+    g.num_kv_heads = p->num_kv_heads;
+    g.capacity = (int32_t)((int64_t)p->pcp_size * p->max_local_blocks * p->block_size);
+    g.head_stride = (int64_t)p->block_size * p->head_dim * es;
+    g.page_stride = 2 * (int64_t)p->num_kv_heads * g.head_stride;
+    return g;
+}
+
+bool misaligned(const pcpa_rows* r) {
+    return ((uintptr_t)r->data & 15u) || (r->token_stride & 7) || (r->head_stride & 7);
+}
+RowsIn rows_in(const pcpa_rows* r) { return RowsIn{(const uint8_t*)r->data, r->token_stride * 2, r->head_stride * 2}; }
+RowsOut rows_out(const pcpa_rows* r) { return RowsOut{(uint8_t*)r->data, r->token_stride * 2, r->head_stride * 2}; }
+
+int32_t check_rotary(const pcpa_params* p, const pcpa_rotary* r) {
+    if (!r) return PCPA_ERR_NULL_POINTER;
+    if (r->rotary_dim < 0 || r->rotary_dim > p->head_dim || r->rotary_dim % 16) return PCPA_ERR_BAD_SHAPE;
+    if (r->rotary_dim > 0 && !r->turns) return PCPA_ERR_NULL_POINTER;
+    if (!isfinite(r->amplitude) || !isfinite(r->norm_eps) || r->norm_eps < 0.f) return PCPA_ERR_BAD_SCALE;
+    const bool f32 = r->weight_dtype == PCPA_DTYPE_FP32;
+    if (!f32 && r->weight_dtype != PCPA_DTYPE_BF16) return PCPA_ERR_BAD_DTYPE;
+    if (((uintptr_t)r->q_weight | (uintptr_t)r->k_weight) & (f32 ? 3u : 1u)) return PCPA_ERR_MISALIGNED;
+    if ((uintptr_t)r->turns & 7u) return PCPA_ERR_MISALIGNED;
+    return PCPA_OK;
+}
+
+void set_rotary(TokenArgs& a, const pcpa_rotary* r) {
+    a.rotary_dim = r->rotary_dim;
+    a.interleaved = r->interleaved ? 1 : 0;
+    a.amplitude = r->amplitude;
+    a.norm_eps = r->norm_eps;
+    a.turns = r->turns;
+    a.q_weight = (const uint8_t*)r->q_weight;
+    a.k_weight = (const uint8_t*)r->k_weight;
+    a.weight_f32 = r->weight_dtype == PCPA_DTYPE_FP32;
+}
+
+template <bool ROTATE, bool PAGES, bool FP8>
+const void* token_kernel_for(int head_dim) {
+    return head_dim == 64    ? (const void*)token_kernel<64, ROTATE, PAGES, FP8>
+           : head_dim == 128 ? (const void*)token_kernel<128, ROTATE, PAGES, FP8>
+                             : (const void*)token_kernel<256, ROTATE, PAGES, FP8>;
+}
+
+constexpr int kWavesInFlight = 256 * 16;
+
+int32_t launch_tokens(const void* fn, TokenArgs& a, const pcpa_params* p, hipStream_t stream) {
+    a.num_q_heads = p->num_q_heads;
+    a.num_kv_heads = p->num_kv_heads;
+    a.rows_per_token = (a.q.data ? p->num_q_heads : 0) + (a.k.data ? p->num_kv_heads : 0) +
+                       (a.v.data ? p->num_kv_heads : 0);
+    const int rows = 64 / (p->head_dim / 8), groups = (a.rows_per_token + rows - 1) / rows;
+    // a wave takes several groups of a token's rows once there are enough
+    // waves for the GPU without
+    const int64_t each = (int64_t)a.chunk.num_tokens * groups / kWavesInFlight;
+    a.groups_per_wave = (int)(each < 1 ? 1 : each > groups ? groups : each);
+    a.waves_per_token = (groups + a.groups_per_wave - 1) / a.groups_per_wave;
+    const int64_t waves = (int64_t)a.chunk.num_tokens * a.waves_per_token, per = kTokenThreads / 64;
+    const int64_t blocks = (waves + per - 1) / per;
+    if (waves > INT32_MAX - per) return PCPA_ERR_TOO_LARGE;
+    void* args[] = {&a};
+    return hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(kTokenThreads), args, 0, stream) == hipSuccess
+               ? PCPA_OK
+               : PCPA_ERR_LAUNCH;
+}
+
+// pcpa_chunk_write, or with a rotation pcpa_chunk_prepare.
+int32_t write_chunk(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary* r, const pcpa_rows* q,
+                    const pcpa_rows* k, const pcpa_rows* v, const pcpa_rows* q_out, const void* block_table,
+                    void* kv_pages, float* token_scales, hipStream_t stream) {
+    int32_t st = check_chunk(p, c);
+    if (st != PCPA_OK) return st;
+    if (r && (st = check_rotary(p, r)) != PCPA_OK) return st;
+    if (!c->lengths || !k || !v || !k->data || !v->data) return PCPA_ERR_NULL_POINTER;
+    if (r && (!q || !q_out || !q->data || !q_out->data)) return PCPA_ERR_NULL_POINTER;
+    if ((st = check_pages(p, block_table, kv_pages, token_scales)) != PCPA_OK) return st;
+    if (misaligned(k) || misaligned(v) || (r && (misaligned(q) || misaligned(q_out)))) return PCPA_ERR_MISALIGNED;
+    if (c->num_tokens == 0) return PCPA_OK;
+    TokenArgs a{};
+    a.chunk = desc_of(c);
+    a.pages = pages_of(p, c->interleave, block_table);
+    a.k = rows_in(k);
+    a.v = rows_in(v);
+    if (r) {
+        a.q = rows_in(q);
+        a.q_out = rows_out(q_out);
+        set_rotary(a, r);
+    }
+    a.position_kind = kOfChunk;
+    a.pool = (uint8_t*)kv_pages;
+    a.token_scales = token_scales;
+    a.k_scale = p->k_scale;
+    a.v_scale = p->v_scale;
+    const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
+    const int d = p->head_dim;
+    const void* const fn = r ? (fp8 ? token_kernel_for<true, true, true>(d) : token_kernel_for<true, true, false>(d))
+                             : (fp8 ? token_kernel_for<false, true, true>(d) : token_kernel_for<false, true, false>(d));
+    return launch_tokens(fn, a, p, stream);
+}
+
+}  // namespace
+}  // namespace chunk
+}  // namespace pcpa
+
+extern "C" {
+
+int32_t pcpa_rotate(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary* r, const void* positions,
+                    int32_t position_bits, int64_t first_pos, const pcpa_rows* q, const pcpa_rows* k,
+                    const pcpa_rows* v, const pcpa_rows* q_out, const pcpa_rows* k_out, const pcpa_rows* v_out,
+                    int32_t striped, void* stream) {
+    using namespace pcpa::chunk;
+    int32_t st = check_chunk(p, c);
+    if (st != PCPA_OK) return st;
+    if ((st = check_rotary(p, r)) != PCPA_OK) return st;
+    if (!q || !k || !q_out || !k_out || !q->data || !k->data || !q_out->data || !k_out->data)
+        return PCPA_ERR_NULL_POINTER;
+    if ((v == nullptr) != (v_out == nullptr) || (v && (!v->data || !v_out->data))) return PCPA_ERR_NULL_POINTER;
+    if (position_bits != kOfChunk && position_bits != kFromFirst && position_bits != kInt32 && position_bits != kInt64)
+        return PCPA_ERR_BAD_SHAPE;
+    const bool given = position_bits > 0;
+    if (given != (positions != nullptr) || (position_bits == kOfChunk && !c->lengths)) return PCPA_ERR_NULL_POINTER;
+    if (position_bits == kFromFirst && (c->batch != 1 || first_pos < 0 || first_pos > INT64_MAX - c->num_tokens))
+        return PCPA_ERR_BAD_SHAPE;
+    if (striped && (position_bits == kOfChunk || c->num_tokens % (p->pcp_size * c->interleave)))
+        return PCPA_ERR_BAD_SHAPE;
+    if (misaligned(q) || misaligned(k) || misaligned(k_out) || ((uintptr_t)q_out->data & 15u) ||
+        (!striped && misaligned(q_out)) || (v && (misaligned(v) || misaligned(v_out))))
+        return PCPA_ERR_MISALIGNED;
+    if ((uintptr_t)positions & (position_bits == kInt64 ? 7u : 3u)) return PCPA_ERR_MISALIGNED;
+    if (c->num_tokens == 0) return PCPA_OK;
+    TokenArgs a{};
+    a.chunk = desc_of(c);
+    a.pages.pcp = p->pcp_size;
+    a.pages.interleave = c->interleave;
+    a.q = rows_in(q);
+    a.k = rows_in(k);
+    a.q_out = rows_out(q_out);
+    a.k_out = rows_out(k_out);
+    if (v) {
+        a.v = rows_in(v);
+        a.v_out = rows_out(v_out);
+    }
+    a.striped = striped ? 1 : 0;
+    a.local_q = c->num_tokens / p->pcp_size;
+    a.position_kind = position_bits;
+    a.positions = positions;
+    a.first_pos = first_pos;
+    set_rotary(a, r);
+    return launch_tokens(token_kernel_for<true, false, false>(p->head_dim), a, p, (hipStream_t)stream);
+}
+
+int32_t pcpa_chunk_write(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rows* k, const pcpa_rows* v,
+                         const void* block_table, void* kv_pages, float* token_scales, void* stream) {
+    return pcpa::chunk::write_chunk(p, c, nullptr, nullptr, k, v, nullptr, block_table, kv_pages, token_scales,
+                                    (hipStream_t)stream);
+}
+
+int32_t pcpa_chunk_prepare(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary* r, const pcpa_rows* q,
+                           const pcpa_rows* k, const pcpa_rows* v, const pcpa_rows* q_out, const void* block_table,
+                           void* kv_pages, float* token_scales, void* stream) {
+    if (!r) return PCPA_ERR_NULL_POINTER;
+    return pcpa::chunk::write_chunk(p, c, r, q, k, v, q_out, block_table, kv_pages, token_scales,
+                                    (hipStream_t)stream);
+}
+
+int32_t pcpa_cache_read(const pcpa_params* p, int32_t interleave, int64_t first_pos, int32_t num_tokens,
+                        const void* block_table, const void* kv_pages, const float* token_scales, void* k, void* v,
+                        void* stream) {
+    using namespace pcpa::chunk;
+    const pcpa_chunk c{interleave, 1, num_tokens, 0, nullptr, nullptr};
+    int32_t st = check_chunk(p, &c);
+    if (st != PCPA_OK) return st;
+    if (first_pos < 0 || first_pos > INT64_MAX - num_tokens) return PCPA_ERR_BAD_SHAPE;
+    if (!k || !v) return PCPA_ERR_NULL_POINTER;
+    if ((st = check_pages(p, block_table, kv_pages, token_scales)) != PCPA_OK) return st;
+    if (((uintptr_t)k | (uintptr_t)v) & 15u) return PCPA_ERR_MISALIGNED;
+    if (num_tokens == 0) return PCPA_OK;
+    ReadArgs a{};
+    a.pages = pages_of(p, interleave, block_table);
+    a.pool = (const uint8_t*)kv_pages;
+    a.token_scales = token_scales;
+    a.k = (uint8_t*)k;
+    a.v = (uint8_t*)v;
+    a.first_pos = first_pos;
+    a.num_tokens = num_tokens;
+    a.k_scale = p->k_scale;
+    a.v_scale = p->v_scale;
+    const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
+    const void* const fn = p->head_dim == 64    ? (fp8 ? (const void*)cache_read_kernel<64, true>
+                                                       : (const void*)cache_read_kernel<64, false>)
+                           : p->head_dim == 128 ? (fp8 ? (const void*)cache_read_kernel<128, true>
+                                                       : (const void*)cache_read_kernel<128, false>)
+                                                : (fp8 ? (const void*)cache_read_kernel<256, true>
+                                                       : (const void*)cache_read_kernel<256, false>);
+    const int64_t blocks = ((int64_t)num_tokens * (p->head_dim / 8) + kTokenThreads - 1) / kTokenThreads;
+    if (blocks > INT32_MAX || p->num_kv_heads > 65535) return PCPA_ERR_TOO_LARGE;
+    void* args[] = {&a};
+    return hipLaunchKernel(fn, dim3((unsigned)blocks, p->num_kv_heads, 2), dim3(kTokenThreads), args, 0,
+                           (hipStream_t)stream) == hipSuccess
+               ? PCPA_OK
+               : PCPA_ERR_LAUNCH;
+}
+
+int64_t pcpa_chunk_workspace_bytes(const pcpa_params* p, const pcpa_chunk* c) {
+    return pcpa::chunk::check_chunk(p, c);
+}
+
+int32_t pcpa_chunk_attention(const pcpa_params* p, const pcpa_chunk* c, const void* q, const void* kv_pages,
+                             const float* token_scales, const void* block_table, void* out, float* lse,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace pcpa::chunk;
+    int32_t st = check_chunk(p, c);
+    if (st != PCPA_OK) return st;
+    if (!c->lengths || !q || !out) return PCPA_ERR_NULL_POINTER;
+    if ((st = check_pages(p, block_table, kv_pages, token_scales)) != PCPA_OK) return st;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15u) return PCPA_ERR_MISALIGNED;
+    if ((uintptr_t)lse & 3u) return PCPA_ERR_MISALIGNED;
+    if (workspace_bytes < 0) return PCPA_ERR_WORKSPACE;
+    if (p->num_q_heads > 65535) return PCPA_ERR_TOO_LARGE;
+    if (c->num_tokens == 0) return PCPA_OK;
+    AttendArgs a{};
+    a.chunk = desc_of(c);
+    a.pages = pages_of(p, c->interleave, block_table);
+    a.q = (const uint8_t*)q;
+    a.pool = (const uint8_t*)kv_pages;
+    a.token_scales = token_scales;
+    a.out = (uint8_t*)out;
+    a.lse = lse;
+    a.num_q_heads = p->num_q_heads;
+    a.group = p->num_q_heads / p->num_kv_heads;
+    a.score_scale = p->softmax_scale * p->k_scale * pcpa::kLog2e;
+    a.v_scale = p->v_scale;
+    const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
+    const void* const fn = p->head_dim == 64    ? (fp8 ? (const void*)attend_rows_kernel<64, true>
+                                                       : (const void*)attend_rows_kernel<64, false>)
+                           : p->head_dim == 128 ? (fp8 ? (const void*)attend_rows_kernel<128, true>
+                                                       : (const void*)attend_rows_kernel<128, false>)
+                                                : (fp8 ? (const void*)attend_rows_kernel<256, true>
+                                                       : (const void*)attend_rows_kernel<256, false>);
+    void* args[] = {&a};
+    return hipLaunchKernel(fn, dim3(c->num_tokens, p->num_q_heads), dim3(64), args, 0, (hipStream_t)stream) ==
+                   hipSuccess
+               ? PCPA_OK
+               : PCPA_ERR_LAUNCH;
+}
+
+}  // extern "C"

@@ -362,6 +362,130 @@ int32_t pcpa_block_mask_valid_len(const void* mask, int32_t pcp_size, int32_t ma
 int32_t pcpa_page_alloc(const pcpa_params* params, int32_t interleave, int64_t first_pos, int32_t num_tokens,
                         void* block_table, const int32_t* free_pages, int32_t* free_count, void* stream);
 
+/*
+ * ---- Serving: sequences that grow over a paged cache -------------------------
+ *
+ * A chunk: the new tokens of `batch` sequences, packed one sequence after
+ * another into num_tokens rows.  Sequence b owns rows [starts[b],
+ * starts[b + 1]); its cache holds positions [0, lengths[b]), the new tokens
+ * the last of them: its row i is position lengths[b] - n_b + i, n_b its number
+ * of rows.  starts NULL: num_tokens / batch rows each (a whole number).  A
+ * sequence may have no row; rows before starts[0] or from starts[batch] on
+ * belong to none and are neither read nor written.  lengths and starts are
+ * device memory, read when the kernels run; starts must not decrease (a bad
+ * value gives wrong rows, never an access out of bounds).
+ * Each sequence's pages are its own [pcp_size, max_local_blocks] slice of the
+ * block table [batch, pcp_size, max_local_blocks], its positions striped over
+ * pcp_size ranks with `interleave` as for pcpa_kv_cache_write (pcp_size 1: an
+ * ordinary paged cache); the pages are those of one pool.
+ */
+typedef struct pcpa_chunk {
+    int32_t interleave;
+    int32_t batch;
+    int32_t num_tokens;
+    int32_t reserved;       /* 0 */
+    const int32_t* lengths; /* device int32 [batch] */
+    const int32_t* starts;  /* device int32 [batch + 1], or NULL */
+} pcpa_chunk;
+
+/* Rows [num_tokens, heads, head_dim] of bf16 values, strides in elements (a
+ * head's head_dim values are contiguous).  data and both strides times 2 bytes
+ * are multiples of 16 bytes. */
+typedef struct pcpa_rows {
+    void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} pcpa_rows;
+
+/*
+ * Norm and rotation of a row x [head_dim]:
+ *   y = x / sqrt(mean(x^2) + norm_eps) * weight      (only where a weight is given)
+ *   pairs (a, b) of the first rotary_dim values, i = 0 .. rotary_dim / 2 - 1:
+ *   (y[i], y[i + rotary_dim / 2]), or (y[2 i], y[2 i + 1]) when interleaved, go to
+ *   amplitude * (a cos - b sin, b cos + a sin) at 2 pi * position * turns[i]
+ * The angle is formed in 64 bits and reduced before it is rounded, the rest in
+ * 32 bits, the result rounded once.
+ */
+typedef struct pcpa_rotary {
+    int32_t rotary_dim;     /* multiple of 16, at most head_dim; 0: no rotation */
+    int32_t interleaved;    /* 0: pairs (i, i + rotary_dim / 2); 1: (2 i, 2 i + 1) */
+    int32_t weight_dtype;   /* PCPA_DTYPE_BF16, or PCPA_DTYPE_FP32 */
+    float amplitude;        /* finite */
+    float norm_eps;         /* finite, not negative */
+    const double* turns;    /* device [rotary_dim / 2]: revolutions per position */
+    const void* q_weight;   /* device [head_dim], or NULL: Q is not normed */
+    const void* k_weight;
+} pcpa_rotary;
+#define PCPA_DTYPE_FP32 3
+
+/*
+ * Norms and rotation of the new tokens' Q and K, out of place or in place
+ * (q_out / k_out the same rows as q / k).
+ * Positions, one of: `positions` (device int32 [num_tokens], or int64 with
+ * position_bits 64; position_bits 32 otherwise), the chunk's own (positions
+ * NULL, position_bits 0), or first_pos + row (position_bits -1; the chunk's
+ * lengths and starts are not read then, batch must be 1).
+ * striped != 0: q_out is the contiguous [pcp_size, num_q_heads, num_tokens /
+ * pcp_size, head_dim] of pcpa_history_attention, row i at the place of current
+ * position i (num_tokens a multiple of pcp_size * interleave; q_out strides are
+ * not read); needs position_bits -1 or positions.
+ * v, v_out (optional, both or neither): V's rows copied to their place.
+ * params: heads and head_dim are used, the rest is validated only.
+ */
+int32_t pcpa_rotate(const pcpa_params* params, const pcpa_chunk* chunk, const pcpa_rotary* rotary,
+                    const void* positions, int32_t position_bits, int64_t first_pos, const pcpa_rows* q,
+                    const pcpa_rows* k, const pcpa_rows* v, const pcpa_rows* q_out, const pcpa_rows* k_out,
+                    const pcpa_rows* v_out, int32_t striped, void* stream);
+
+/*
+ * The new tokens' K and V into their sequences' pages.
+ *   token_scales  NULL, or (e4m3 pools) float [num_pages, 2, num_kv_heads,
+ *                 block_size]: a row x of token and head is stored as
+ *                 round_e4m3(x / s), s = max(max_d |x_d| / 448, 2^-80) over its
+ *                 finite values, and s written to the row's place (K: 0, V: 1);
+ *                 values that are not finite become NaN codes.  params' k_scale
+ *                 and v_scale must be 1.  NULL: as pcpa_kv_cache_write.
+ * Rows whose position is negative or beyond the cache, or whose table entry is
+ * outside [0, num_pages), are not written.
+ */
+int32_t pcpa_chunk_write(const pcpa_params* params, const pcpa_chunk* chunk, const pcpa_rows* k, const pcpa_rows* v,
+                         const void* block_table, void* kv_pages, float* token_scales, void* stream);
+
+/*
+ * pcpa_rotate (positions: the chunk's own) and pcpa_chunk_write of the rotated K
+ * and of V in one launch, with the same results.
+ */
+int32_t pcpa_chunk_prepare(const pcpa_params* params, const pcpa_chunk* chunk, const pcpa_rotary* rotary,
+                           const pcpa_rows* q, const pcpa_rows* k, const pcpa_rows* v, const pcpa_rows* q_out,
+                           const void* block_table, void* kv_pages, float* token_scales, void* stream);
+
+/*
+ * Positions [first_pos, first_pos + num_tokens) of one sequence's cache as bf16
+ * values: code * scale (token_scales, or params' k_scale / v_scale), rounded
+ * once.  block_table [pcp_size, max_local_blocks]; k, v [num_kv_heads,
+ * num_tokens, head_dim].  Positions beyond the cache, or whose table entry is
+ * outside [0, num_pages), give zeros.
+ */
+int32_t pcpa_cache_read(const pcpa_params* params, int32_t interleave, int64_t first_pos, int32_t num_tokens,
+                        const void* block_table, const void* kv_pages, const float* token_scales, void* k, void* v,
+                        void* stream);
+
+/*
+ * Causal attention of a chunk's rows over their sequences' caches, which hold
+ * the chunk's K and V already: the row at position p sees positions 0 .. p.
+ *   q, out  [num_tokens, num_q_heads, head_dim] bf16
+ *   lse     float [num_tokens, num_q_heads] or NULL: as pcpa_history_attention_lse
+ * A row that sees nothing (a negative position, no page) gets zeros and -inf.
+ * Both products run on bf16 operands (e4m3 codes widened exactly, the scales
+ * applied in 32 bits).  Long walks are cut into ranges when there are few rows;
+ * their partials go to `workspace`, device memory of pcpa_chunk_workspace_bytes
+ * bytes, 16-byte aligned, which needs no initialisation; NULL if that is 0.
+ */
+int64_t pcpa_chunk_workspace_bytes(const pcpa_params* params, const pcpa_chunk* chunk);
+int32_t pcpa_chunk_attention(const pcpa_params* params, const pcpa_chunk* chunk, const void* q, const void* kv_pages,
+                             const float* token_scales, const void* block_table, void* out, float* lse,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
