@@ -1,14 +1,29 @@
 // Causal attention of new tokens over the paged caches of their sequences.
 #pragma once
 
+#include "cache_kernels.hpp"
 #include "chunk_common.hpp"
 
 namespace pcpa {
 namespace chunk {
 
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
+constexpr int kTileKeys = 64;  // keys of a walk's tile: a whole number of them to a page
+
+// What the merge needs to find a sequence's partial results: written by the
+// sequence's first workgroup.
+struct SequencePlan {
+    int32_t first_item;  // of all its (KV head, range, row tile) items, row tile fastest
+    int32_t ranges;      // its walk is cut into; 1: results are final
+    int32_t tiles;       // row tiles
+    int32_t rows;        // rows of a row tile
+};
+
 struct AttendArgs {
     Desc chunk;
     Pages pages;
+    cache::FastDiv div_pcp, div_block;
     const uint8_t* q;
     const uint8_t* pool;
     const float* token_scales;
@@ -16,76 +31,673 @@ struct AttendArgs {
     float* lse;
     int32_t num_q_heads;
     int32_t group;
-    float score_scale;  // softmax_scale * k_scale * log2(e)
+    int32_t max_items;     // the launch's workgroups
+    int32_t slots;         // workgroups that the GPU holds at once
+    int32_t min_range;     // tiles a range has at least
+    float score_scale;     // softmax_scale * k_scale * log2(e)
     float v_scale;
+    float* part_o;         // [max_items, rows, D] fp32 normalised outputs of ranges
+    float* part_lse;       // [max_items, rows] log2 of their sums
+    SequencePlan* plans;   // [batch]
 };
 
-template <bool FP8>
-__device__ __forceinline__ float cached(const uint8_t* row, int d) {
-    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(row[d], 0);
-    return bf16_bits_to_f32(((const uint16_t*)row)[d]);
+// One workgroup's share: row tile `tile` of sequence b and KV head `head`, the
+// walk's tiles [begin, end).
+struct Item {
+    int b, head, tile, range;
+    int begin, end;
+    SequencePlan plan;
+    Span span;
+    int length;  // of the cache, clamped to what it holds
+};
+
+// Tiles of the walk over positions [0, keys): rank by rank within each 64 local
+// positions, so that with chunks of 64 they follow the positions.  Tile i is
+// local positions 64 (i / pcp) .. of rank i % pcp; a few may be empty.
+__device__ __forceinline__ int walk_tiles(const Pages& p, int keys) {
+    const int most = (int)paging::owned_below(keys, 0, p.pcp, p.interleave);
+    return p.pcp * ((most + kTileKeys - 1) / kTileKeys);
 }
 
-// One wave per (row, Q head): scores of 64 keys at a time, a key to a lane, with
-// a running maximum m and sum l (s in log2 units, p = 2^(s - m)); then the lanes
-// take D / 64 values of the output each and go through the 64 probabilities.
-template <int D, bool FP8>
-__global__ void __launch_bounds__(64) attend_rows_kernel(AttendArgs a) {
-    constexpr int PER = D / 64, ES = FP8 ? 1 : 2;
-    const int lane = threadIdx.x;
+// The item of workgroup `index`; false when there is none.  Every wave of the
+// workgroup finds it by itself, 64 sequences at a time: first the work of the
+// whole chunk, which gives the tiles a range should have so that all ranges
+// fill the GPU once, then the sequence that the index falls into.  (A launch
+// of its own for this took longer than the scan: two dependent loads and a few
+// shuffles for up to 64 sequences.)
+__device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int rows_per_tile, Item& it) {
+    const int lane = threadIdx.x & 63, heads = a.pages.num_kv_heads;
+    auto sequence = [&](int base, Span& span, int& length, int& tiles, int& walk) {
+        span = Span{0, 0};
+        length = tiles = walk = 0;
+        if (base + lane < a.chunk.batch) {
+            span = span_of(a.chunk, base + lane);
+            length = min(max(a.chunk.lengths[base + lane], 0), a.pages.capacity);
+            tiles = (int)(((int64_t)span.count * a.group + rows_per_tile - 1) / rows_per_tile);
+            // (a sequence whose rows see nothing still has an item, for their zeros)
+            walk = max(walk_tiles(a.pages, length), 1);
+        }
+    };
+    Span span, first_span;
+    int length, tiles, walk, first_length, first_tiles, first_walk;
+    int64_t work = 0;
+    for (int base = 0; base < a.chunk.batch; base += 64) {
+        sequence(base, span, length, tiles, walk);
+        if (base == 0) {
+            first_span = span;
+            first_length = length;
+            first_tiles = tiles;
+            first_walk = walk;
+        }
+        work += (int64_t)tiles * walk;
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) work += __shfl_xor(work, off);
+    const int64_t share = (work * heads + a.slots - 1) / a.slots;
+    const int range = (int)max(share, (int64_t)a.min_range);
+    int before = 0;
+    for (int base = 0; base < a.chunk.batch; base += 64) {
+        if (base == 0) {
+            span = first_span;
+            length = first_length;
+            tiles = first_tiles;
+            walk = first_walk;
+        } else {
+            sequence(base, span, length, tiles, walk);
+        }
+        const int ranges = (walk + range - 1) / range;
+        const int items = tiles * heads * ranges;
+        int incl = items;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int up = __shfl_up(incl, off);
+            if (lane >= off) incl += up;
+        }
+        const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > index);
+        if (past) {
+            const int src = __builtin_ctzll(past);
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
+            it.b = base + src;
+            it.span = Span{of(span.first), of(span.count)};
+            it.length = of(length);
+            it.plan = SequencePlan{before + of(incl) - of(items), of(ranges), of(tiles), rows_per_tile};
+            int at = index - it.plan.first_item;
+            const int per_head = it.plan.ranges * it.plan.tiles;
+            it.head = at / per_head;
+            at -= it.head * per_head;
+            it.range = at / it.plan.tiles;
+            it.tile = at - it.range * it.plan.tiles;
+            // (starts that decrease may overflow the sums: no such item)
+            if (at < 0 || it.head >= heads || it.range >= it.plan.ranges) return false;
+            const int w = of(walk);
+            it.begin = (int)((int64_t)w * it.range / it.plan.ranges);
+            it.end = (int)((int64_t)w * (it.range + 1) / it.plan.ranges);
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return false;
+}
+
+__device__ __forceinline__ float quarters_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// ---- few rows ------------------------------------------------------------------
+//
+// For up to 32 rows per (sequence, KV head) - one token of a GQA group, or a few
+// - the work is reading the cache once: every wave streams its own keys, no wave
+// waits for another.  A step of a wave is KEYS keys:
+//   * S^T = K Q^T by 16x16x32 MFMAs.  K goes from the pages straight into the A
+//     operand's registers: lane 16 g + r holds 16 bytes of the key in row r, four
+//     lanes 64 bytes in a row, and Q's registers hold the same values of d in the
+//     same order (the order of a sum of products is free).  Row r of tile t is key
+//     8 (r / 4) + 4 t + r % 4 of 32, so that the scores of lane group g, (t, i),
+//     are keys 8 g + 4 t + i: the B operand of the next product as they stand.
+//   * the running maximum m, sum l and O^T of each row stay in registers; m is
+//     raised only when a step exceeds it by 2^8 (as in the tile kernel).
+//   * O^T += V^T P^T.  V goes into the wave's own LDS by DMA, 16-byte chunks
+//     swizzled by key so that the transposing reads find every bank once.
+// The next step's K (registers) and V (LDS) load while this one is computed: 16
+// KB (e4m3) or 32 KB (bf16) in flight per wave, 128 KB per CU.  The waves' results
+// meet in LDS at the end.
+template <int D, bool FP8, int RT>
+struct FewShape {
+    static constexpr int ROW = D * (FP8 ? 1 : 2);    // bytes of a key's row
+    static constexpr int KG = D == 256 ? 1 : 2;      // 32-key groups of a step
+    static constexpr int KEYS = 32 * KG;
+    static constexpr int SUB = kTileKeys / KEYS;     // steps of a tile
+    static constexpr int KC = ROW / 64;              // 16-byte loads of a K row per lane
+    static constexpr int QK = D / 32;                // k-steps of the score MFMA
+    static constexpr int DT = D / 16;
+    static constexpr int V_BYTES = KEYS * ROW;
+    static constexpr int V_BLOCKS = V_BYTES / 1024;  // DMA instructions of a step
+    static constexpr int CH = ROW / 16;              // 16-byte chunks of a row
+    // eight waves where their registers (256 each) and LDS hold it
+    static constexpr int WAVES = (D == 256 && (!FP8 || RT == 2)) || (D == 128 && !FP8) ? 4 : 8;
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int O_ROW = D + 4;              // floats: 16 rows then start in all banks
+    static constexpr int V_LDS = WAVES * 2 * V_BYTES;
+    static constexpr int O_LDS = WAVES * 16 * O_ROW * 4;
+    static constexpr int LDS = V_LDS > O_LDS ? V_LDS : O_LDS;
+    static constexpr int PER_CU = D == 64 && FP8 && RT == 1 ? 2 : 1;  // workgroups that fit
+    static constexpr int ROWS = 16 * RT;
+};
+
+// Chunk swizzle of V's rows in LDS.  A transposing read of 8-bit values takes
+// 16 keys x 16 bytes at once, one of 16-bit values 8 keys (0-3 and 8-11, or 4
+// more) x 32 bytes: the keys of either then lie in different 16-byte (32-byte)
+// parts of the 256 bytes that the banks span.
+template <int ROW, bool FP8>
+__device__ __forceinline__ constexpr int few_swizzle(int key) {
+    constexpr int CH = ROW / 16;
+    if constexpr (FP8) return (key / (256 / ROW)) & (CH < 16 ? CH - 1 : 15);
+    if constexpr (CH == 8) return 2 * (((key >> 1) & 1) | ((key >> 2) & 2));
+    return 2 * ((key & 3) | ((key >> 1) & 4));
+}
+
+template <class S>
+struct FewStep {
+    int n;        // keys of it that some row may see
+    int rank;
+    int local;    // the rank's local position of its first key
+    int page;     // -1: no step
+    int slot;
+    int u;
+};
+
+template <class S>
+struct FewLoads {
+    v4i k[2 * S::KG * S::KC];             // free once the scores are there
+    v4f ks[2 * S::KG], vs[2 * S::KG];     // the keys' scales
+};
+
+template <int D, bool FP8, bool SCALED, int RT>
+__global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
+                                  (FewShape<D, FP8, RT>::PER_CU * FewShape<D, FP8, RT>::WAVES / 4))
+    attend_few_kernel(AttendArgs a) {
+    using S = FewShape<D, FP8, RT>;
+    constexpr int ROW = S::ROW, KG = S::KG, KC = S::KC, DT = S::DT, QK = S::QK;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::LDS];
+    __shared__ float wave_ml[S::WAVES][16][2];
+
+    Item it;
+    if (!find_item(a, blockIdx.x, S::ROWS, it)) return;
+    if (it.head == 0 && it.tile == 0 && it.range == 0 && threadIdx.x == 0 && a.plans) a.plans[it.b] = it.plan;
+
+    const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rows = it.span.count * a.group;
+
+    // ---- this lane's rows: Q operand and the positions they see ---------------
+    v8bf qop[RT][QK];
+    int seen[RT];  // positions [0, seen) of the sequence
+    const int row0 = it.tile * S::ROWS;
+    // the tile's last row sees the most
+    const int last = min(row0 + S::ROWS, rows) - 1;
+    const int64_t len = a.chunk.lengths[it.b];
+    auto sees = [&](int row) {
+        const int64_t np = len - it.span.count + row / a.group + 1;
+        return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
+    };
+    const int most = __builtin_amdgcn_readfirstlane(sees(last)), least = __builtin_amdgcn_readfirstlane(sees(row0));
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = row0 + 16 * rt + r16;
+        const bool ok = row < rows;
+        seen[rt] = ok ? sees(row) : most;  // rows past the last mask nothing
+        const int tok = it.span.first + row / a.group, hd = it.head * a.group + row % a.group;
+        const uint8_t* const qrow = a.q + ((int64_t)tok * a.num_q_heads + hd) * D * 2;
+#pragma unroll
+        for (int c = 0; c < QK; ++c) {
+            const int d = FP8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
+            v4i x{0, 0, 0, 0};
+            if (ok) x = *(const v4i*)(qrow + d * 2);
+            qop[rt][c] = __builtin_bit_cast(v8bf, x);
+        }
+    }
+    // striping: whole rounds and the rest of what each row sees
+    const int stride = a.pages.pcp * a.pages.interleave;
+    int rounds[RT], rest[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        rounds[rt] = seen[rt] / stride * a.pages.interleave;
+        rest[rt] = seen[rt] % stride;
+    }
+    const int most_rounds = most / stride * a.pages.interleave, most_rest = most % stride;
+    const int least_rounds = least / stride * a.pages.interleave, least_rest = least % stride;
+    auto owned = [&](int whole, int tail, int rank) {
+        return whole + min(max(tail - rank * a.pages.interleave, 0), a.pages.interleave);
+    };
+
+    // ---- the wave's steps ----------------------------------------------------------
+    typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
+    const const_i32_ptr table = (const_i32_ptr)(a.pages.table + (table_of(a.pages, it.b) << a.pages.table_shift));
+    const int steps = (it.end - it.begin) * S::SUB;
+    // The wave's first step from step u on that has keys; page -1 past the last.
+    // (Steps without keys are passed over here, in scalar code: a loop body that
+    // may be skipped had two copies of O^T and K in registers.)
+    auto step_from = [&](int u) {
+        FewStep<S> s{0, 0, 0, -1, 0, u};
+        for (; s.u < steps; s.u += S::WAVES) {
+            const uint32_t tile = it.begin + s.u / S::SUB;
+            const uint32_t lt = cache::div(tile, a.div_pcp);
+            const int rank = tile - lt * a.pages.pcp;
+            const int local = lt * kTileKeys + (s.u % S::SUB) * S::KEYS;
+            const int n = min(owned(most_rounds, most_rest, rank) - local, S::KEYS);
+            const uint32_t blk = cache::div(local, a.div_block);
+            if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
+            const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
+            if ((unsigned)page >= (unsigned)a.pages.num_pages) continue;
+            s.n = __builtin_amdgcn_readfirstlane(n);
+            s.rank = __builtin_amdgcn_readfirstlane(rank);
+            s.local = __builtin_amdgcn_readfirstlane(local);
+            s.page = __builtin_amdgcn_readfirstlane(page);
+            s.slot = __builtin_amdgcn_readfirstlane(local - (int)blk * a.pages.block_size);
+            break;
+        }
+        return s;
+    };
+
+    uint8_t* const my_lds = lds + wave * 2 * S::V_BYTES;
+    const uint32_t my_addr = lds_address(my_lds);
+    const uint32_t k_lane = (8 * (r16 >> 2) + (r16 & 3)) * ROW + 16 * g;
+    // lane's chunk of DMA block 0: LDS chunk `lane` holds the swizzled one.  Block
+    // i's keys differ in bits that the lane does not set: their part of the
+    // swizzle is a constant.
+    uint32_t v_lane;
+    {
+        const int key = lane / S::CH, c = lane % S::CH;
+        v_lane = key * ROW + ((c ^ few_swizzle<ROW, FP8>(key)) << 4);
+    }
+    // transposing reads: this lane's address of d tile 0, 32-key group 0
+    uint32_t v_read[FP8 ? 1 : 2];
+    if constexpr (FP8) {
+        const int key = 8 * g + (r16 >> 1);
+        v_read[0] = my_addr + key * ROW + (few_swizzle<ROW, FP8>(key) << 4) + 8 * (r16 & 1);
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int key = 8 * g + 4 * s + (r16 >> 2), byte = 8 * (r16 & 3);
+            v_read[s] = my_addr + key * ROW + (((byte >> 4) ^ few_swizzle<ROW, FP8>(key)) << 4) + (byte & 15);
+        }
+    }
+    const uint8_t* const k_pool = a.pool + it.head * a.pages.head_stride;
+    const int64_t v_offset = a.pages.num_kv_heads * a.pages.head_stride;
+    const float* const k_scales = a.token_scales + (int64_t)it.head * a.pages.block_size;
+    const int64_t vs_offset = (int64_t)a.pages.num_kv_heads * a.pages.block_size;
+    FewLoads<S> L;
+    auto issue_v = [&](const FewStep<S>& s, uint32_t dst) {
+        if (s.page < 0) return;
+        const uint8_t* const vb = k_pool + s.page * a.pages.page_stride + s.slot * ROW + v_offset;
+        // (opaque, here and below: addresses that differ by a constant are formed
+        // when they are used, not kept in registers for the whole walk)
+        uint32_t off = v_lane;
+        asm volatile("" : "+v"(off));
+        static_for<0, S::V_BLOCKS>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            dma_sbase<0>(vb + 1024 * i, off ^ (few_swizzle<ROW, FP8>(64 * i / S::CH) << 4), dst + 1024 * i);
+        });
+    };
+    auto issue_k = [&](const FewStep<S>& s) {
+        if (s.page < 0) return;
+        const uint8_t* const kb = k_pool + s.page * a.pages.page_stride + s.slot * ROW + k_lane;
+#pragma unroll
+        for (int t = 0; t < 2 * KG; ++t)
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+                L.k[t * KC + c] = *(const v4i*)(kb + ((t >> 1) * 32 + (t & 1) * 4) * ROW + c * 64);
+    };
+    auto issue_scales = [&](const FewStep<S>& s) {
+        if (!SCALED || s.page < 0) return;
+        const float* const sc = k_scales + (int64_t)s.page * 2 * vs_offset + s.slot + 8 * g;
+#pragma unroll
+        for (int t = 0; t < 2 * KG; ++t) {
+            L.ks[t] = *(const v4f*)(sc + (t >> 1) * 32 + (t & 1) * 4);
+            L.vs[t] = *(const v4f*)(sc + vs_offset + (t >> 1) * 32 + (t & 1) * 4);
+        }
+    };
+
+    float m[RT], l[RT];
+    v4f o[RT][DT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = -1.0e30f;  // (finite: a step may be hidden from a row before any that is not)
+        l[rt] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[rt][dt] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // ---- the walk: the step after next is looked up, the next loads, this one runs ----
+    FewStep<S> st = step_from(wave), nxt = step_from(st.u + S::WAVES);
+    issue_v(st, my_addr);
+    issue_k(st);
+    issue_scales(st);
+    uint32_t buf = 0;
+    while (st.page >= 0) {
+        wait_vmem();
+        __builtin_amdgcn_sched_barrier(0);
+        issue_v(nxt, my_addr + (buf ^ S::V_BYTES));
+        const FewStep<S> after = step_from(nxt.u + S::WAVES);
+        // ---- scores -----------------------------------------------------------
+        v4f s[RT][2 * KG];
+#pragma unroll
+        for (int t = 0; t < 2 * KG; ++t) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt][t] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < QK; ++c) {
+                v8bf kop;
+                if constexpr (FP8) {
+                    const v4i x = L.k[t * KC + (c >> 1)];
+                    kop = __builtin_bit_cast(v8bf, e4m3x8_to_bf16x8(x[2 * (c & 1)], x[2 * (c & 1) + 1]));
+                } else {
+                    kop = __builtin_bit_cast(v8bf, L.k[t * KC + c]);
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop, qop[rt][c], s[rt][t], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        issue_k(nxt);
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- V's rows that not every row sees, or none -----------------------------
+        const int all = owned(least_rounds, least_rest, st.rank) - st.local;  // keys that every row sees
+        if (all < S::KEYS) {
+            uint8_t* const vt = my_lds + buf;
+            // A value that is not finite would reach rows that do not see its key,
+            // as 0 times it: such values are added to the rows that do, and
+            // cleared before the product.
+            for (int key = max(all, 0); key < st.n; ++key) {
+                static_for<0, DT>([&](auto dc) {
+                    constexpr int dt = decltype(dc)::value;
+                    const int byte = (16 * dt + 4 * g) * (FP8 ? 1 : 2);
+                    uint8_t* const at = vt + key * ROW + (((byte >> 4) ^ few_swizzle<ROW, FP8>(key)) << 4) + (byte & 15);
+                    float v[4];
+                    if constexpr (FP8) {
+                        const int w = *(const int*)at;
+                        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+                        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+                        v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
+                    } else {
+                        const v2i w = *(const v2i*)at;
+                        v[0] = bf16_bits_to_f32((uint32_t)w[0] & 0xffffu), v[1] = bf16_bits_to_f32((uint32_t)w[0] >> 16);
+                        v[2] = bf16_bits_to_f32((uint32_t)w[1] & 0xffffu), v[3] = bf16_bits_to_f32((uint32_t)w[1] >> 16);
+                    }
+                    bool bad = false;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bad |= !(fabsf(v[i]) < INFINITY);
+                    if (__builtin_amdgcn_ballot_w64(bad)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool hit = !(fabsf(v[i]) < INFINITY);
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+                                if (hit && key < owned(rounds[rt], rest[rt], st.rank) - st.local) o[rt][dt][i] += v[i];
+                            if (hit && r16 == 0) {
+                                if constexpr (FP8)
+                                    at[i] = 0;
+                                else
+                                    ((uint16_t*)at)[i] = 0;
+                            }
+                        }
+                    }
+                });
+            }
+            for (int i = st.n * S::CH + lane; i < S::KEYS * S::CH; i += 64) *(v4i*)(vt + i * 16) = v4i{0, 0, 0, 0};
+            asm volatile("" ::: "memory");
+            if constexpr (SCALED) {  // (nor do the scales of slots without a token mean anything)
+#pragma unroll
+                for (int t = 0; t < 2 * KG; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        L.vs[t][i] = 32 * (t >> 1) + 4 * (t & 1) + i < st.n - 8 * g ? L.vs[t][i] : 0.f;
+            }
+        }
+        // ---- softmax ---------------------------------------------------------------
+        v8bf pop[RT][KG];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int vis = owned(rounds[rt], rest[rt], st.rank) - st.local;
+#pragma unroll
+            for (int t = 0; t < 2 * KG; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[rt][t][i] *= SCALED ? L.ks[t][i] * a.score_scale : a.score_scale;
+            if (all < S::KEYS) {
+#pragma unroll
+                for (int t = 0; t < 2 * KG; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        s[rt][t][i] = 32 * (t >> 1) + 4 * (t & 1) + i < vis - 8 * g ? s[rt][t][i] : -INFINITY;
+            }
+            float mx = s[rt][0][0];
+#pragma unroll
+            for (int t = 0; t < 2 * KG; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][t][i]);
+            mx = quarters_max(mx);
+            const bool raise = mx > m[rt] + 8.f;
+            if (__builtin_amdgcn_ballot_w64(raise)) {
+                const float next = raise ? mx : m[rt];
+                const float keep = raise ? __builtin_amdgcn_exp2f(m[rt] - next) : 1.f;
+                l[rt] *= keep;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= keep;
+                m[rt] = next;
+            }
+#pragma unroll
+            for (int t = 0; t < 2 * KG; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(s[rt][t][i] - m[rt]);
+                    l[rt] += p;
+                    // (one rounding: 2^-8 of each probability, of either sign)
+                    pop[rt][t >> 1][4 * (t & 1) + i] = (__bf16)(SCALED ? p * L.vs[t][i] : p);
+                }
+        }
+        issue_scales(nxt);
+        // ---- O^T += V^T P^T -----------------------------------------------------------
+        constexpr int READS = DT * KG;  // operands: d tile dt of 32-key group kg
+        uint32_t va[FP8 ? 1 : 2];
+#pragma unroll
+        for (int i = 0; i < (FP8 ? 1 : 2); ++i) {
+            va[i] = v_read[i] + buf;
+            asm volatile("" : "+v"(va[i]));
+        }
+        if constexpr (FP8) {
+            v2i x[2][4];
+            auto read4 = [&](auto nc) {
+                constexpr int n = decltype(nc)::value;
+                static_for<0, 4>([&](auto ec) {
+                    constexpr int op = 4 * n + decltype(ec)::value, dt = op / KG, kg = op % KG;
+                    x[n & 1][decltype(ec)::value] =
+                        ds_read_tr8_b64<kg * 32 * ROW>(va[0] ^ (dt << 4));
+                });
+            };
+            read4(std::integral_constant<int, 0>{});
+            static_for<0, READS / 4>([&](auto nc) {
+                constexpr int n = decltype(nc)::value;
+                lds_results_ready(x[n & 1]);
+                if constexpr (n + 1 < READS / 4) read4(std::integral_constant<int, n + 1>{});
+                static_for<0, 4>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value, op = 4 * n + e, dt = op / KG, kg = op % KG;
+                    const v8bf vop = __builtin_bit_cast(v8bf, e4m3x8_to_bf16x8(x[n & 1][e][0], x[n & 1][e][1]));
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rt][kg], o[rt][dt], 0, 0, 0);
+                });
+            });
+        } else {
+            v2i x[2][4];  // two operands of two reads
+            auto read2 = [&](auto nc) {
+                constexpr int n = decltype(nc)::value;
+                static_for<0, 2>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value, op = 2 * n + e, dt = op / KG, kg = op % KG;
+                    constexpr int off = kg * 32 * ROW;
+                    x[n & 1][2 * e] = ds_read_tr16_b64<off>(va[0] ^ (dt << 5));
+                    x[n & 1][2 * e + 1] = ds_read_tr16_b64<off>(va[1] ^ (dt << 5));
+                });
+            };
+            read2(std::integral_constant<int, 0>{});
+            static_for<0, READS / 2>([&](auto nc) {
+                constexpr int n = decltype(nc)::value;
+                lds_results_ready(x[n & 1]);
+                if constexpr (n + 1 < READS / 2) read2(std::integral_constant<int, n + 1>{});
+                static_for<0, 2>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value, op = 2 * n + e, dt = op / KG, kg = op % KG;
+                    const v4i w{x[n & 1][2 * e][0], x[n & 1][2 * e][1], x[n & 1][2 * e + 1][0], x[n & 1][2 * e + 1][1]};
+                    const v8bf vop = __builtin_bit_cast(v8bf, w);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rt][kg], o[rt][dt], 0, 0, 0);
+                });
+            });
+        }
+        st = nxt;
+        nxt = after;
+        buf ^= S::V_BYTES;
+    }
+
+    // ---- the waves' results meet: 16 rows at a time ---------------------------------
+    float* const ol = (float*)lds;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float sum = quarters_sum(l[rt]);
+        __syncthreads();  // every wave is done with its part of the LDS
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+            *(v4f*)(ol + (wave * 16 + r16) * S::O_ROW + 16 * dt + 4 * g) = o[rt][dt];
+        if (g == 0) {
+            wave_ml[wave][r16][0] = m[rt];
+            wave_ml[wave][r16][1] = sum;
+        }
+        __syncthreads();
+        for (int i = tid; i < 16 * (D / 4); i += S::THREADS) {
+            const int j = i / (D / 4), c = i % (D / 4), row = row0 + 16 * rt + j;
+            if (row >= rows) continue;
+            float top = wave_ml[0][j][0];
+#pragma unroll
+            for (int w = 1; w < S::WAVES; ++w) top = fmaxf(top, wave_ml[w][j][0]);
+            float total = 0.f;
+            v4f acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < S::WAVES; ++w) {
+                const float weight = __builtin_amdgcn_exp2f(wave_ml[w][j][0] - top);
+                total = fmaf(weight, wave_ml[w][j][1], total);
+                const v4f x = *(const v4f*)(ol + (w * 16 + j) * S::O_ROW + 4 * c);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[k] = fmaf(weight, x[k], acc[k]);
+            }
+            // (a row that sees nothing: zeros.  NaN sums divide to NaN)
+            const bool empty = total == 0.f;
+            const float inv = empty ? 0.f : a.v_scale / total;
+            const float log2sum = empty ? -INFINITY : top + __builtin_amdgcn_logf(total);
+            if (it.plan.ranges > 1) {
+                const int64_t prow = (int64_t)blockIdx.x * S::ROWS + 16 * rt + j;
+                *(v4f*)(a.part_o + prow * D + 4 * c) = empty ? v4f{0.f, 0.f, 0.f, 0.f} : acc * inv;
+                if (c == 0) a.part_lse[prow] = log2sum;
+            } else {
+                const int tok = it.span.first + row / a.group, hd = it.head * a.group + row % a.group;
+                const int64_t at = (int64_t)tok * a.num_q_heads + hd;
+                uint32_t w[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const __bf16 lo = (__bf16)(empty ? 0.f : acc[2 * k] * inv), hi = (__bf16)(empty ? 0.f : acc[2 * k + 1] * inv);
+                    w[k] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+                }
+                *(v2i*)(a.out + (at * D + 4 * c) * 2) = v2i{(int)w[0], (int)w[1]};
+                if (a.lse && c == 0) a.lse[at] = log2sum * kLn2;
+            }
+        }
+    }
+}
+
+// ---- ranges of one walk ----------------------------------------------------------
+
+// One workgroup per (row, Q head): the partial results of the ranges of the
+// row's walk, weighted by their sums.  D / 4 threads take a partial's values,
+// THREADS / (D / 4) partials at a time.
+template <int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) merge_ranges_kernel(AttendArgs a) {
+    constexpr int LANES = D / 4, AT_ONCE = THREADS / LANES;
+    __shared__ v4f part[AT_ONCE][LANES];
+    __shared__ float part_ml[AT_ONCE][2];
     const int token = blockIdx.x, head = blockIdx.y, kv = head / a.group;
     const int b = sequence_of(a.chunk, token);
     if (b < 0) return;
+    const SequencePlan plan = a.plans[b];
+    if (plan.ranges <= 1 || plan.rows <= 0) return;
     const Span span = span_of(a.chunk, b);
-    const int64_t pos = (int64_t)a.chunk.lengths[b] - span.count + (token - span.first);
-    const int64_t table = table_of(a.pages, b);
-    const int64_t at = (int64_t)token * a.num_q_heads + head;
-    const uint16_t* const q = (const uint16_t*)(a.q + at * D * 2);
-    const int64_t k_off = kv * a.pages.head_stride, v_off = (a.pages.num_kv_heads + kv) * a.pages.head_stride;
-    const int64_t keys = pos + 1 < a.pages.capacity ? pos + 1 : a.pages.capacity;
-    float m = -INFINITY, l = 0.f, o[PER] = {};
-    for (int64_t base = 0; base < keys; base += 64) {
-        const Place p = base + lane < keys ? place_of(a.pages, table, base + lane) : Place{-1, 0};
-        float s = -INFINITY, vs = a.v_scale;
-        if (p.page >= 0) {
-            const uint8_t* const row = a.pool + p.page * a.pages.page_stride + k_off + (int64_t)p.slot * D * ES;
-            float dot = 0.f;
-            for (int d = 0; d < D; ++d) dot = fmaf(bf16_bits_to_f32(q[d]), cached<FP8>(row, d), dot);
-            if (a.token_scales) {
-                const float* const sc = a.token_scales + ((int64_t)p.page * 2 * a.pages.num_kv_heads + kv) *
-                                                             a.pages.block_size + p.slot;
-                dot *= sc[0];
-                vs *= sc[(int64_t)a.pages.num_kv_heads * a.pages.block_size];
-            }
-            s = dot * a.score_scale;
+    const int row = (token - span.first) * a.group + (head - kv * a.group);
+    const int tile = row / plan.rows;
+    const int64_t first = (int64_t)plan.first_item + (int64_t)kv * plan.ranges * plan.tiles + tile;
+    // (only starts that decrease lead past the launch's items)
+    if (plan.first_item < 0 || tile >= plan.tiles || first + (int64_t)(plan.ranges - 1) * plan.tiles >= a.max_items)
+        return;
+    const int at = threadIdx.x / LANES, c = threadIdx.x % LANES;
+    float top = -INFINITY, total = 0.f;
+    v4f acc{0.f, 0.f, 0.f, 0.f};
+    constexpr int UNROLL = 4;
+    for (int s0 = at; s0 < plan.ranges; s0 += AT_ONCE * UNROLL) {
+        float ls[UNROLL];
+        v4f x[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int s = s0 + u * AT_ONCE;
+            const int64_t prow = (first + (int64_t)min(s, plan.ranges - 1) * plan.tiles) * plan.rows + row % plan.rows;
+            ls[u] = s < plan.ranges ? a.part_lse[prow] : -INFINITY;
+            x[u] = *(const v4f*)(a.part_o + prow * D + 4 * c);
         }
-        float top = s;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-        const float next = fmaxf(m, top);
-        const float weight = p.page >= 0 ? exp2f(s - next) : 0.f;
-        float sum = weight;
+        for (int u = 0; u < UNROLL; ++u) {
+            if (ls[u] == -INFINITY) continue;  // nothing seen in it, or past the last range
+            const float next = fmaxf(top, ls[u]);
+            const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+            const float weight = __builtin_amdgcn_exp2f(ls[u] - next);
+            total = fmaf(total, keep, weight);
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-        const float keep = m == -INFINITY ? 0.f : exp2f(m - next);
-        l = l * keep + sum;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] *= keep;
-        m = next;
-        for (int k = 0; k < 64; ++k) {
-            const int page = __shfl(p.page, k), slot = __shfl(p.slot, k);
-            const float w = __shfl(weight * vs, k);
-            if (page < 0) continue;
-            const uint8_t* const row = a.pool + page * a.pages.page_stride + v_off + (int64_t)slot * D * ES;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) o[i] = fmaf(w, cached<FP8>(row, lane * PER + i), o[i]);
+            for (int k = 0; k < 4; ++k) acc[k] = fmaf(acc[k], keep, weight * x[u][k]);
+            top = next;
         }
     }
-    const bool seen = m != -INFINITY;
-    __bf16* const out = (__bf16*)(a.out + at * D * 2);
+    part[at][c] = acc;
+    if (c == 0) {
+        part_ml[at][0] = top;
+        part_ml[at][1] = total;
+    }
+    __syncthreads();
+    if (at != 0) return;
+    top = part_ml[0][0];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) out[lane * PER + i] = (__bf16)(seen ? o[i] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[at] = seen ? m * kLn2 + logf(l) : -INFINITY;
+    for (int p = 1; p < AT_ONCE; ++p) top = fmaxf(top, part_ml[p][0]);
+    total = 0.f;
+    acc = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < AT_ONCE; ++p) {
+        if (part_ml[p][1] == 0.f) continue;  // nothing seen (a NaN is not nothing)
+        const float weight = __builtin_amdgcn_exp2f(part_ml[p][0] - top);
+        total = fmaf(weight, part_ml[p][1], total);
+        const v4f x = part[p][c];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = fmaf(weight, x[k], acc[k]);
+    }
+    const bool empty = total == 0.f;
+    const float inv = empty ? 0.f : 1.f / total;
+    const int64_t out_row = (int64_t)token * a.num_q_heads + head;
+    uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const __bf16 lo = (__bf16)(empty ? 0.f : acc[2 * k] * inv), hi = (__bf16)(empty ? 0.f : acc[2 * k + 1] * inv);
+        w[k] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+    }
+    *(v2i*)(a.out + (out_row * D + 4 * c) * 2) = v2i{(int)w[0], (int)w[1]};
+    if (a.lse && c == 0) a.lse[out_row] = empty ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
 }  // namespace chunk

@@ -18,7 +18,8 @@ int32_t check_chunk(const pcpa_params* p, const pcpa_chunk* c) {
     if (!c->starts && c->num_tokens % c->batch) return PCPA_ERR_BAD_SHAPE;
     if (((uintptr_t)c->lengths | (uintptr_t)c->starts) & 3u) return PCPA_ERR_MISALIGNED;
     const int64_t capacity = (int64_t)p->pcp_size * p->max_local_blocks * p->block_size;
-    if (capacity > INT32_MAX || (int64_t)p->pcp_size * c->interleave > INT32_MAX ||
+    // (256: room for the walk's rounding up)
+    if (capacity > INT32_MAX - 256ll * p->pcp_size || (int64_t)p->pcp_size * c->interleave > INT32_MAX ||
         (int64_t)c->num_tokens * p->num_q_heads > INT32_MAX)
         return PCPA_ERR_TOO_LARGE;
     return PCPA_OK;
@@ -148,6 +149,116 @@ int32_t write_chunk(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary
     return launch_tokens(fn, a, p, stream);
 }
 
+// ---- attention ---------------------------------------------------------------
+
+struct AttendKernel {
+    const void* fn;
+    int threads, rows, per_cu;
+};
+// (a kernel with and without token scales has the same shape)
+template <int D, bool FP8, int RT>
+AttendKernel few_kernel(bool scaled) {
+    using S = FewShape<D, FP8, RT>;
+    return AttendKernel{scaled ? (const void*)attend_few_kernel<D, FP8, FP8, RT>
+                               : (const void*)attend_few_kernel<D, FP8, false, RT>,
+                        S::THREADS, S::ROWS, S::PER_CU};
+}
+template <bool FP8, int RT>
+AttendKernel few_kernel_for(int d, bool scaled) {
+    return d == 64    ? few_kernel<64, FP8, RT>(scaled)
+           : d == 128 ? few_kernel<128, FP8, RT>(scaled)
+                      : few_kernel<256, FP8, RT>(scaled);
+}
+
+constexpr int kCUs = 256;  // MI355X
+// A range of a walk has at least this many tiles (64 keys each).
+constexpr int kMinRange = 8;
+
+struct AttendPlan {
+    AttendKernel kernel;
+    int64_t items;        // workgroups of the launch
+    bool ranges;          // walks may be cut into ranges
+    int64_t part_lse, plans, bytes;
+};
+
+AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = false) {
+    AttendPlan w{};
+    const int64_t group = p->num_q_heads / p->num_kv_heads;
+    const int64_t sequences = c->num_tokens < c->batch ? c->num_tokens : c->batch;
+    const bool narrow = sequences > 0 && c->num_tokens * group <= 16 * sequences;
+    const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
+    const int d = p->head_dim;
+    w.kernel = fp8 ? (narrow ? few_kernel_for<true, 1>(d, scaled) : few_kernel_for<true, 2>(d, scaled))
+                   : (narrow ? few_kernel_for<false, 1>(d, false) : few_kernel_for<false, 2>(d, false));
+    // row tiles of one KV head: at most one that is not full per sequence
+    const int64_t tiles = c->num_tokens * group / w.kernel.rows + sequences;
+    const int64_t slots = (int64_t)kCUs * w.kernel.per_cu;
+    w.ranges = c->num_tokens > 0 && tiles * p->num_kv_heads < 4 * slots;
+    w.items = tiles * p->num_kv_heads + (w.ranges ? slots : 0);
+    if (w.ranges) {
+        const int64_t rows = w.items * w.kernel.rows;
+        w.part_lse = rows * d * 4;
+        w.plans = w.part_lse + rows * 4;
+        w.bytes = w.plans + (int64_t)c->batch * sizeof(SequencePlan);
+    }
+    return w;
+}
+
+template <int D>
+const void* merge_kernel_for(bool wide) {
+    return wide ? (const void*)merge_ranges_kernel<D, 1024> : (const void*)merge_ranges_kernel<D, 256>;
+}
+
+int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const void* kv_pages,
+               const float* token_scales, const void* block_table, void* out, float* lse, void* workspace,
+               int64_t workspace_bytes, hipStream_t stream) {
+    int32_t st = check_chunk(p, c);
+    if (st != PCPA_OK) return st;
+    if (!c->lengths || !q || !out) return PCPA_ERR_NULL_POINTER;
+    if ((st = check_pages(p, block_table, kv_pages, token_scales)) != PCPA_OK) return st;
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15u) return PCPA_ERR_MISALIGNED;
+    if ((uintptr_t)lse & 3u) return PCPA_ERR_MISALIGNED;
+    const AttendPlan w = attend_plan(p, c, token_scales != nullptr);
+    if (workspace_bytes < 0 || (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes))) return PCPA_ERR_WORKSPACE;
+    if (p->num_q_heads > 65535 || w.items > INT32_MAX / 64) return PCPA_ERR_TOO_LARGE;
+    if (c->num_tokens == 0) return PCPA_OK;
+    AttendArgs a{};
+    a.chunk = desc_of(c);
+    a.pages = pages_of(p, c->interleave, block_table);
+    a.div_pcp = cache::make_fastdiv((uint32_t)p->pcp_size);
+    a.div_block = cache::make_fastdiv((uint32_t)p->block_size);
+    a.q = (const uint8_t*)q;
+    a.pool = (const uint8_t*)kv_pages;
+    a.token_scales = token_scales;
+    a.out = (uint8_t*)out;
+    a.lse = lse;
+    a.num_q_heads = p->num_q_heads;
+    a.group = p->num_q_heads / p->num_kv_heads;
+    a.max_items = (int32_t)w.items;
+    a.slots = kCUs * w.kernel.per_cu;
+    a.min_range = w.ranges ? kMinRange : 1 << 30;  // (beyond any walk)
+    a.score_scale = p->softmax_scale * p->k_scale * kLog2e;
+    a.v_scale = p->v_scale;
+    if (w.ranges) {
+        a.part_o = (float*)workspace;
+        a.part_lse = (float*)((uint8_t*)workspace + w.part_lse);
+        a.plans = (SequencePlan*)((uint8_t*)workspace + w.plans);
+    }
+    void* args[] = {&a};
+    if (hipLaunchKernel(w.kernel.fn, dim3((unsigned)w.items), dim3(w.kernel.threads), args, 0, stream) != hipSuccess)
+        return PCPA_ERR_LAUNCH;
+    if (!w.ranges) return PCPA_OK;
+    // few rows: many ranges each, taken by 16 waves
+    const bool wide = (int64_t)c->num_tokens * p->num_q_heads <= kCUs;
+    const void* const merge = p->head_dim == 64    ? merge_kernel_for<64>(wide)
+                              : p->head_dim == 128 ? merge_kernel_for<128>(wide)
+                                                   : merge_kernel_for<256>(wide);
+    return hipLaunchKernel(merge, dim3(c->num_tokens, p->num_q_heads), dim3(wide ? 1024 : 256), args, 0, stream) ==
+                   hipSuccess
+               ? PCPA_OK
+               : PCPA_ERR_LAUNCH;
+}
+
 }  // namespace
 }  // namespace chunk
 }  // namespace pcpa
@@ -252,46 +363,15 @@ int32_t pcpa_cache_read(const pcpa_params* p, int32_t interleave, int64_t first_
 }
 
 int64_t pcpa_chunk_workspace_bytes(const pcpa_params* p, const pcpa_chunk* c) {
-    return pcpa::chunk::check_chunk(p, c);
+    const int32_t st = pcpa::chunk::check_chunk(p, c);
+    return st == PCPA_OK ? pcpa::chunk::attend_plan(p, c).bytes : st;
 }
 
 int32_t pcpa_chunk_attention(const pcpa_params* p, const pcpa_chunk* c, const void* q, const void* kv_pages,
                              const float* token_scales, const void* block_table, void* out, float* lse,
                              void* workspace, int64_t workspace_bytes, void* stream) {
-    using namespace pcpa::chunk;
-    int32_t st = check_chunk(p, c);
-    if (st != PCPA_OK) return st;
-    if (!c->lengths || !q || !out) return PCPA_ERR_NULL_POINTER;
-    if ((st = check_pages(p, block_table, kv_pages, token_scales)) != PCPA_OK) return st;
-    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15u) return PCPA_ERR_MISALIGNED;
-    if ((uintptr_t)lse & 3u) return PCPA_ERR_MISALIGNED;
-    if (workspace_bytes < 0) return PCPA_ERR_WORKSPACE;
-    if (p->num_q_heads > 65535) return PCPA_ERR_TOO_LARGE;
-    if (c->num_tokens == 0) return PCPA_OK;
-    AttendArgs a{};
-    a.chunk = desc_of(c);
-    a.pages = pages_of(p, c->interleave, block_table);
-    a.q = (const uint8_t*)q;
-    a.pool = (const uint8_t*)kv_pages;
-    a.token_scales = token_scales;
-    a.out = (uint8_t*)out;
-    a.lse = lse;
-    a.num_q_heads = p->num_q_heads;
-    a.group = p->num_q_heads / p->num_kv_heads;
-    a.score_scale = p->softmax_scale * p->k_scale * pcpa::kLog2e;
-    a.v_scale = p->v_scale;
-    const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
-    const void* const fn = p->head_dim == 64    ? (fp8 ? (const void*)attend_rows_kernel<64, true>
-                                                       : (const void*)attend_rows_kernel<64, false>)
-                           : p->head_dim == 128 ? (fp8 ? (const void*)attend_rows_kernel<128, true>
-                                                       : (const void*)attend_rows_kernel<128, false>)
-                                                : (fp8 ? (const void*)attend_rows_kernel<256, true>
-                                                       : (const void*)attend_rows_kernel<256, false>);
-    void* args[] = {&a};
-    return hipLaunchKernel(fn, dim3(c->num_tokens, p->num_q_heads), dim3(64), args, 0, (hipStream_t)stream) ==
-                   hipSuccess
-               ? PCPA_OK
-               : PCPA_ERR_LAUNCH;
+    return pcpa::chunk::attend(p, c, q, kv_pages, token_scales, block_table, out, lse, workspace, workspace_bytes,
+                               (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -66,6 +66,9 @@ CASES = {
     "prompts": (dict(d=128, hq=16, hkv=2, block=64), [129, 1, 64, 300, 257], [129, 1, 64, 300, 257]),
     "prompts_fp8_d256": (dict(d=256, kv=FP8, hq=32, hkv=2, block=128), [200, 65], [200, 65]),
     "prompts_fp8_d64": (dict(d=64, kv=FP8, hq=24, hkv=8, block=64), [200, 65], [200, 65]),
+    # rows enough to fill the GPU several times over (walks are not cut into ranges)
+    "many_rows": (dict(d=64, hq=32, hkv=2, bucket=640), [600, 520, 1], [600, 520, 1]),
+    "many_rows_fp8": (dict(d=128, kv=FP8, hq=32, hkv=2, bucket=1280), [640, 1280, 3], [500, 620, 1]),
     # more new tokens than the cache holds (rows that see nothing), empty caches
     "empty_rows": (dict(d=128, hq=8, hkv=2), [5, 0, 0, 130], [9, 3, 0, 131]),
     "empty_rows_fp8": (dict(d=256, kv=FP8, hq=32, hkv=2), [2, 0], [4, 1]),
