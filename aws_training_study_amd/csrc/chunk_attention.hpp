@@ -3,6 +3,7 @@
 
 #include "cache_kernels.hpp"
 #include "chunk_common.hpp"
+#include "tile_kernel.hpp"
 
 namespace pcpa {
 namespace chunk {
@@ -14,7 +15,7 @@ constexpr int kTileKeys = 64;  // keys of a walk's tile: a whole number of them 
 // What the merge needs to find a sequence's partial results: written by the
 // sequence's first workgroup.
 struct SequencePlan {
-    int32_t first_item;  // of all its (KV head, range, row tile) items, row tile fastest
+    int32_t first_item;  // of all its (range, row tile from the last on, KV head) items, KV head fastest
     int32_t ranges;      // its walk is cut into; 1: results are final
     int32_t tiles;       // row tiles
     int32_t rows;        // rows of a row tile
@@ -122,13 +123,14 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
             it.length = of(length);
             it.plan = SequencePlan{before + of(incl) - of(items), of(ranges), of(tiles), rows_per_tile};
             int at = index - it.plan.first_item;
-            const int per_head = it.plan.ranges * it.plan.tiles;
-            it.head = at / per_head;
-            at -= it.head * per_head;
-            it.range = at / it.plan.tiles;
-            it.tile = at - it.range * it.plan.tiles;
+            if (at < 0) return false;
+            const int rest = at / heads;
+            it.head = at - rest * heads;
+            it.range = rest / it.plan.tiles;
+            // the last rows, which see the most, first
+            it.tile = it.plan.tiles - 1 - (rest - it.range * it.plan.tiles);
             // (starts that decrease may overflow the sums: no such item)
-            if (at < 0 || it.head >= heads || it.range >= it.plan.ranges) return false;
+            if (it.range >= it.plan.ranges) return false;
             const int w = of(walk);
             it.begin = (int)((int64_t)w * it.range / it.plan.ranges);
             it.end = (int)((int64_t)w * (it.range + 1) / it.plan.ranges);
@@ -618,6 +620,306 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     }
 }
 
+// ---- many rows -------------------------------------------------------------------
+//
+// For more rows per (sequence, KV head) the products bound: the tile kernel's
+// workgroups of 128 rows (tile_kernel.hpp: K and V tiles shared through LDS, both
+// products on 32x32 MFMAs, bf16 operands), over the walk of this sequence's table
+// and with every row's own last key.
+
+// The sequence's walk for one workgroup: tile i of [begin, end) as find_item
+// counts them.
+struct ManyTile {
+    int i;
+    int page;   // -1: past the last
+    int slot;
+    int n;      // keys that some row may see
+    int rank;
+    int local;
+};
+
+template <int D, bool FP8, bool SCALED>
+__global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShape<D, FP8, false>::PAIR ? 1 : 2))
+    attend_many_kernel(AttendArgs a) {
+    static_assert(!SCALED || FP8, "token scales go with e4m3 caches");
+    using S = TileShape<D, FP8, false>;
+    constexpr int ROW = S::ROW, CHUNKS = S::CHUNKS, QK = S::QK, DT = S::DT;
+    constexpr bool F8 = S::F8, TWO = S::TILES == 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::LDS_BYTES];
+    __shared__ __attribute__((aligned(16))) float scales[SCALED ? 2 * S::TILES * 2 * kKeyTile : 4];
+    __shared__ float pair_ml[S::PAIR ? kWaves * 64 * 2 : 1];
+
+    Item it;
+    if (!find_item(a, blockIdx.x, kRowsPerGroup, it)) return;
+    if (it.head == 0 && it.tile == 0 && it.range == 0 && threadIdx.x == 0 && a.plans) a.plans[it.b] = it.plan;
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pw = S::PAIR ? wave & (kWaves - 1) : wave;  // the wave's 32-row slot
+    const int kh = S::PAIR ? wave / kWaves : 0;           // PAIR: its keys (half a tile, or every second tile)
+    const int j = lane & 31, h = lane >> 5, grp = lane >> 4, gl = lane & 15;
+
+    // ---- this lane's row and what it sees ------------------------------------------
+    const int rows = it.span.count * a.group, row0 = it.tile * kRowsPerGroup;
+    const int row = row0 + pw * kRowsPerWave + j;
+    const bool row_ok = row < rows;
+    const int row_c = min(row, rows - 1);  // rows past the last do as the last, unseen
+    const int64_t len = a.chunk.lengths[it.b];
+    auto sees = [&](int r) {
+        const int64_t np = len - it.span.count + r / a.group + 1;
+        return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
+    };
+    const int64_t row_index = (int64_t)(it.span.first + row_c / a.group) * a.num_q_heads + it.head * a.group + row_c % a.group;
+    const int stride = a.pages.pcp * a.pages.interleave;
+    const int seen = sees(row_c);
+    const int rounds = seen / stride * a.pages.interleave, rest = seen % stride;
+    const int most = __builtin_amdgcn_readfirstlane(sees(min(row0 + kRowsPerGroup, rows) - 1));
+    const int least = __builtin_amdgcn_readfirstlane(sees(row0));
+    const int most_rounds = most / stride * a.pages.interleave, most_rest = most % stride;
+    const int least_rounds = least / stride * a.pages.interleave, least_rest = least % stride;
+    auto owned = [&](int whole, int tail, int rank) {
+        return whole + min(max(tail - rank * a.pages.interleave, 0), a.pages.interleave);
+    };
+    v8bf qop[QK];
+#pragma unroll
+    for (int c = 0; c < QK; ++c) {
+        const int d = S::WIDE ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h;
+        qop[c] = __builtin_bit_cast(v8bf, *(const v4i*)(a.q + (row_index * D + d) * 2));
+    }
+
+    // ---- per-lane LDS and DMA offsets (the tile kernel's maps) ------------------------
+    LaneMap<S> L;
+    {
+        const int r = lds_row<F8>(key_of_row<F8>(0, j));
+        L.k_addr = r * ROW + ((h ^ chunk_swizzle<F8, CHUNKS>(r)) << 4) + (S::PAIR_HALVES ? kh * S::K_T1_ROWS * ROW : 0);
+    }
+    if constexpr (F8) {
+        const int r = lds_row<F8>(32 * (grp >> 1) + (gl >> 1));
+        L.v_addr[0] = lds_address(lds) + r * ROW + (((grp & 1) ^ chunk_swizzle_v<F8, CHUNKS>(r)) << 4) + 8 * (gl & 1);
+    } else {
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+            const int vkey = 8 * (grp >> 1) + 4 * s2 + (gl >> 2);
+            const int dbyte = 2 * (16 * (grp & 1) + 4 * (gl & 3));
+            L.v_addr[s2] = lds_address(lds) + vkey * ROW + (((dbyte >> 4) ^ chunk_swizzle_v<F8, CHUNKS>(vkey)) << 4) +
+                           (dbyte & 15) + kh * 32 * ROW;
+        }
+    }
+    {
+        const int byte = wave * 1024 + lane * 16, r = byte / ROW, pos = (byte % ROW) / 16;
+        L.dma_off = lds_row<F8>(r) * ROW + (pos ^ chunk_swizzle<F8, CHUNKS>(r)) * 16;
+        L.dma_off_v = lds_row<F8>(r) * ROW + (pos ^ chunk_swizzle_v<F8, CHUNKS>(r)) * 16;
+    }
+
+    // ---- the walk ------------------------------------------------------------------------
+    typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
+    const const_i32_ptr table = (const_i32_ptr)(a.pages.table + (table_of(a.pages, it.b) << a.pages.table_shift));
+    const int end = min(it.end, walk_tiles(a.pages, most));
+    auto tile_from = [&](int i) {
+        ManyTile t{i, -1, 0, 0, 0, 0};
+        for (; t.i < end; ++t.i) {
+            const uint32_t lt = cache::div((uint32_t)t.i, a.div_pcp);
+            const int rank = t.i - lt * a.pages.pcp, local = lt * kKeyTile;
+            const int n = min(owned(most_rounds, most_rest, rank) - local, kKeyTile);
+            const uint32_t blk = cache::div((uint32_t)local, a.div_block);
+            if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
+            const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
+            if ((unsigned)page >= (unsigned)a.pages.num_pages) continue;
+            t.n = __builtin_amdgcn_readfirstlane(n);
+            t.rank = __builtin_amdgcn_readfirstlane(rank);
+            t.local = __builtin_amdgcn_readfirstlane(local);
+            t.page = __builtin_amdgcn_readfirstlane(page);
+            t.slot = __builtin_amdgcn_readfirstlane(local - (int)blk * a.pages.block_size);
+            break;
+        }
+        return t;
+    };
+    FwdArgs f{};
+    f.kv = a.pool + it.head * a.pages.head_stride;
+    f.head_stride = a.pages.head_stride;
+    f.num_kv_heads = a.pages.num_kv_heads;
+    // the thread's scale of tile t: threads 0 .. 63 K's, 64 .. 127 V's (TWO: the
+    // next 128 the second tile's); slots without a token hold none
+    auto load_scale = [&](const ManyTile& t, const ManyTile& t2) {
+        const bool other = TWO && (tid & 128);
+        const int page = other ? t2.page : t.page, slot = other ? t2.slot : t.slot, n = other ? t2.n : t.n;
+        const int key = tid & 63, which = (tid >> 6) & 1;
+        if (page < 0 || key >= n || tid >= 128 * S::TILES) return 0.f;
+        return a.token_scales[(((int64_t)page * 2 + which) * a.pages.num_kv_heads + it.head) * a.pages.block_size + slot +
+                              key];
+    };
+
+    SoftmaxState<S> st;
+    st.m = -1.0e30f;  // (finite: a tile may be hidden from a row before any that is not)
+    st.l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) st.o[dt] = v16f{};
+
+    // V rows of a staged tile that not every row sees: no value there may reach
+    // a row that does not, as 0 times it, unless it is finite.  Rows past the n
+    // keys are cleared, and values that are not finite: those join the rows that
+    // see their keys after the walk.  Called by the whole workgroup.
+    bool spoiled = false;
+    auto settle_v = [&](uint8_t* v, const ManyTile& t) {
+        const int from = max(owned(least_rounds, least_rest, t.rank) - t.local, 0);
+        if (t.n < kKeyTile) zero_masked_v<S>(v, t.n, tid);
+        bool bad = false;
+        for (int i = from * CHUNKS + tid; i < t.n * CHUNKS; i += S::THREADS) {
+            v4i* const at = (v4i*)(v + lds_row<F8>(i / CHUNKS) * ROW + (i % CHUNKS) * 16);
+            v4i x = *at;
+            bool here = false;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t u = (uint32_t)x[w];
+                if constexpr (F8) {
+#pragma unroll
+                    for (int b = 0; b < 32; b += 8)
+                        if (((u >> b) & 0x7fu) == 0x7fu) u &= ~(0xffu << b);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 32; b += 16)
+                        if (((u >> b) & 0x7f80u) == 0x7f80u) u &= ~(0xffffu << b);
+                }
+                here |= u != (uint32_t)x[w];
+                x[w] = (int)u;
+            }
+            if (here) *at = x;
+            bad |= here;
+        }
+        spoiled |= __syncthreads_or(bad) != 0;
+    };
+    auto settled = [&](const ManyTile& t) { return owned(least_rounds, least_rest, t.rank) - t.local >= kKeyTile; };
+
+    ManyTile cur = tile_from(it.begin), cur2{}, nxt, nxt2{};
+    float scale = 0.f;
+    auto stage = [&](const ManyTile& t, const ManyTile& t2, uint8_t* buf) {
+        if (t.page >= 0) stage_tile_async<S>(f, TileCursor{0, t.slot, 0, t.page * a.pages.page_stride}, buf, wave, L);
+        if (TWO && t2.page >= 0)
+            stage_tile_async<S>(f, TileCursor{0, t2.slot, 0, t2.page * a.pages.page_stride}, buf + 2 * S::TILE, wave, L);
+        if constexpr (SCALED) scale = load_scale(t, t2);
+    };
+    if constexpr (TWO) cur2 = tile_from(cur.i + 1);
+    stage(cur, cur2, lds);
+    for (int rbuf = 0; cur.page >= 0; rbuf ^= 1) {
+        nxt = tile_from((TWO ? cur2.i : cur.i) + 1);
+        if constexpr (TWO) nxt2 = tile_from(nxt.i + 1);
+        const uint32_t rt_off = rbuf * S::BUFFER;
+        wait_vmem();  // this wave's loads of the current tiles have landed
+        float* const sc = scales + rbuf * S::TILES * 2 * kKeyTile;
+        if (SCALED && tid < 128 * S::TILES) sc[tid] = scale;
+        __syncthreads();  // ... and every wave's; the other buffer is free
+        stage(nxt, nxt2, lds + (rt_off ^ S::BUFFER));
+        if (!settled(cur)) settle_v(lds + rt_off + S::TILE, cur);
+        if (TWO && cur2.page >= 0 && !settled(cur2)) settle_v(lds + rt_off + 3 * S::TILE, cur2);
+        if constexpr (TWO) {
+            const ManyTile& t = kh ? cur2 : cur;
+            if (t.page >= 0)
+                compute_tile<S, 0, true, SCALED>(lds, rt_off + kh * 2 * S::TILE, owned(rounds, rest, t.rank) - t.local,
+                                                 qop, a.score_scale, L, h, st, sc + kh * 2 * kKeyTile);
+        } else {
+            const int first_key = S::PAIR ? 32 * kh : 0;
+            compute_tile<S, 0, true, SCALED>(lds, rt_off, owned(rounds, rest, cur.rank) - cur.local - first_key, qop,
+                                             a.score_scale, L, h, st, sc);
+        }
+        cur = nxt;
+        cur2 = nxt2;
+    }
+
+    // ---- PAIR: the two waves' results meet in the first wave of the pair ----------------
+    if constexpr (S::PAIR) {
+        float* const xo = (float*)lds + pw * (DT * 16 * 64);
+        __syncthreads();
+        if (kh == 1) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4)
+                    *(v4f*)(xo + ((4 * dt + r4) * 64 + lane) * 4) =
+                        v4f{st.o[dt][4 * r4], st.o[dt][4 * r4 + 1], st.o[dt][4 * r4 + 2], st.o[dt][4 * r4 + 3]};
+            pair_ml[(pw * 64 + lane) * 2] = st.m;
+            pair_ml[(pw * 64 + lane) * 2 + 1] = st.l;
+        }
+        __syncthreads();
+        if (kh == 1) return;
+        const float m1 = pair_ml[(pw * 64 + lane) * 2], l1 = pair_ml[(pw * 64 + lane) * 2 + 1];
+        const float m = fmaxf(st.m, m1);
+        const float w0 = __builtin_amdgcn_exp2f(st.m - m), w1 = __builtin_amdgcn_exp2f(m1 - m);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const v4f x = *(const v4f*)(xo + ((4 * dt + r4) * 64 + lane) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st.o[dt][4 * r4 + i] = fmaf(w1, x[i], w0 * st.o[dt][4 * r4 + i]);
+            }
+        st.l = fmaf(w1, l1, w0 * st.l);
+        st.m = m;
+    }
+
+    // ---- values that are not finite, for the rows that see them (from the pages) -----------
+    if (spoiled) {
+        for (ManyTile t = tile_from(it.begin); t.page >= 0; t = tile_from(t.i + 1)) {
+            const int vis = min(owned(rounds, rest, t.rank) - t.local, t.n);
+            for (int key = max(owned(least_rounds, least_rest, t.rank) - t.local, 0); key < t.n; ++key) {
+                const uint8_t* const v = f.kv + t.page * a.pages.page_stride + a.pages.num_kv_heads * a.pages.head_stride +
+                                         (int64_t)(t.slot + key) * ROW + 4 * h * S::ES;
+                if (key >= vis) continue;
+                static_for<0, 4 * DT>([&](auto c) {
+                    constexpr int dt = decltype(c)::value >> 2, r4 = decltype(c)::value & 3;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int d = 32 * dt + 8 * r4 + i;
+                        float x;
+                        if constexpr (F8)
+                            x = (v[d] & 0x7f) == 0x7f ? NAN : 0.f;
+                        else
+                            x = bf16_bits_to_f32(((const uint16_t*)v)[d]);
+                        if (!(fabsf(x) < INFINITY)) st.o[dt][4 * r4 + i] += x;
+                    }
+                });
+            }
+        }
+    }
+
+    // ---- O = O^T / l, or the range's partial result ---------------------------------------
+    const float total = halves_sum(st.l);
+    const bool empty = total == 0.f;
+    const float inv = empty ? 0.f : a.v_scale / total;
+    const float log2sum = empty ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
+    if (!row_ok) return;
+    const bool part = it.plan.ranges > 1;
+    const int64_t prow = (int64_t)blockIdx.x * kRowsPerGroup + pw * kRowsPerWave + j;
+    float* const po = a.part_o + prow * D;
+    uint8_t* const orow = a.out + row_index * D * 2;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int d = 32 * dt + 8 * r4 + 4 * h;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = empty ? 0.f : st.o[dt][4 * r4 + i] * inv;
+            if (part) {
+                *(v4f*)(po + d) = v4f{x[0], x[1], x[2], x[3]};
+            } else {
+                uint32_t w[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const __bf16 lo = (__bf16)x[2 * k], hi = (__bf16)x[2 * k + 1];
+                    w[k] = (uint32_t)__builtin_bit_cast(uint16_t, lo) |
+                           ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+                }
+                *(v2i*)(orow + 2 * d) = v2i{(int)w[0], (int)w[1]};
+            }
+        }
+    if (h == 0) {
+        if (part)
+            a.part_lse[prow] = log2sum;
+        else if (a.lse)
+            a.lse[row_index] = log2sum * kLn2;
+    }
+}
+
 // ---- ranges of one walk ----------------------------------------------------------
 
 // One workgroup per (row, Q head): the partial results of the ranges of the
@@ -636,10 +938,10 @@ __global__ void __launch_bounds__(THREADS) merge_ranges_kernel(AttendArgs a) {
     const Span span = span_of(a.chunk, b);
     const int row = (token - span.first) * a.group + (head - kv * a.group);
     const int tile = row / plan.rows;
-    const int64_t first = (int64_t)plan.first_item + (int64_t)kv * plan.ranges * plan.tiles + tile;
+    const int64_t heads = a.pages.num_kv_heads, first = plan.first_item + (plan.tiles - 1 - tile) * heads + kv;
+    const int64_t step = plan.tiles * heads;
     // (only starts that decrease lead past the launch's items)
-    if (plan.first_item < 0 || tile >= plan.tiles || first + (int64_t)(plan.ranges - 1) * plan.tiles >= a.max_items)
-        return;
+    if (plan.first_item < 0 || tile >= plan.tiles || first + (plan.ranges - 1) * step >= a.max_items) return;
     const int at = threadIdx.x / LANES, c = threadIdx.x % LANES;
     float top = -INFINITY, total = 0.f;
     v4f acc{0.f, 0.f, 0.f, 0.f};
@@ -650,7 +952,7 @@ __global__ void __launch_bounds__(THREADS) merge_ranges_kernel(AttendArgs a) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int s = s0 + u * AT_ONCE;
-            const int64_t prow = (first + (int64_t)min(s, plan.ranges - 1) * plan.tiles) * plan.rows + row % plan.rows;
+            const int64_t prow = (first + min(s, plan.ranges - 1) * step) * plan.rows + row % plan.rows;
             ls[u] = s < plan.ranges ? a.part_lse[prow] : -INFINITY;
             x[u] = *(const v4f*)(a.part_o + prow * D + 4 * c);
         }

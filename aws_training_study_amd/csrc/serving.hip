@@ -170,6 +170,18 @@ AttendKernel few_kernel_for(int d, bool scaled) {
                       : few_kernel<256, FP8, RT>(scaled);
 }
 
+template <int D, bool FP8>
+AttendKernel many_kernel(bool scaled) {
+    using S = TileShape<D, FP8, false>;
+    return AttendKernel{scaled ? (const void*)attend_many_kernel<D, FP8, FP8>
+                               : (const void*)attend_many_kernel<D, FP8, false>,
+                        S::THREADS, kRowsPerGroup, S::PAIR ? 1 : 2};
+}
+template <bool FP8>
+AttendKernel many_kernel_for(int d, bool scaled) {
+    return d == 64 ? many_kernel<64, FP8>(scaled) : d == 128 ? many_kernel<128, FP8>(scaled) : many_kernel<256, FP8>(scaled);
+}
+
 constexpr int kCUs = 256;  // MI355X
 // A range of a walk has at least this many tiles (64 keys each).
 constexpr int kMinRange = 8;
@@ -188,8 +200,10 @@ AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = 
     const bool narrow = sequences > 0 && c->num_tokens * group <= 16 * sequences;
     const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
     const int d = p->head_dim;
-    w.kernel = fp8 ? (narrow ? few_kernel_for<true, 1>(d, scaled) : few_kernel_for<true, 2>(d, scaled))
-                   : (narrow ? few_kernel_for<false, 1>(d, false) : few_kernel_for<false, 2>(d, false));
+    const bool many = c->num_tokens * group > 32 * sequences;
+    w.kernel = many  ? (fp8 ? many_kernel_for<true>(d, scaled) : many_kernel_for<false>(d, false))
+               : fp8 ? (narrow ? few_kernel_for<true, 1>(d, scaled) : few_kernel_for<true, 2>(d, scaled))
+                     : (narrow ? few_kernel_for<false, 1>(d, false) : few_kernel_for<false, 2>(d, false));
     // row tiles of one KV head: at most one that is not full per sequence
     const int64_t tiles = c->num_tokens * group / w.kernel.rows + sequences;
     const int64_t slots = (int64_t)kCUs * w.kernel.per_cu;

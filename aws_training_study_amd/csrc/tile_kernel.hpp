@@ -135,10 +135,14 @@ using QOperand = typename std::conditional<S::MFMA8, v8i, v8bf>::type;
 //
 // rt_off: a byte offset added to both buffers' addresses at run time (PAIR
 // walks alternate buffers with one loop body, BUF 0; otherwise 0).
-template <class S, int BUF, bool CAUSAL = false>
+// SCALED (e4m3 tiles): `scales` in LDS holds the tile's 64 K scales, then its 64
+// V scales: a key's scores are multiplied by its K scale, its probabilities by
+// its V scale before they meet V.
+template <class S, int BUF, bool CAUSAL = false, bool SCALED = false>
 __device__ __forceinline__ void compute_tile(const uint8_t* lds, uint32_t rt_off, int valid,
                                              const QOperand<S> (&qop)[S::QK], float cscale,
-                                             const LaneMap<S>& L, int h, SoftmaxState<S>& st) {
+                                             const LaneMap<S>& L, int h, SoftmaxState<S>& st,
+                                             const float* scales = nullptr) {
     constexpr bool F8 = S::F8, FP8 = S::MFMA8;
     constexpr int ROW = S::ROW, QK = S::QK, DT = S::DT;
     constexpr int KBASE = BUF * S::BUFFER;
@@ -218,6 +222,17 @@ __device__ __forceinline__ void compute_tile(const uint8_t* lds, uint32_t rt_off
     // (the two waves of one pair on a SIMD) when the wave at its MFMAs does
     // (64-rank BF16 cache 16.43 vs 16.62 ms; interleaved runs on one box).
     __builtin_amdgcn_s_setprio(S::PAIR ? 0 : 1);
+    if constexpr (SCALED) {
+        static_assert(S::WIDE, "scales go with e4m3 tiles and bf16 MFMAs");
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const v4f x = *(const v4f*)(scales + key_of_acc<F8>(t, 4 * r4, h));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][4 * r4 + i] *= x[i];
+            }
+    }
     // ---- mask, online softmax (lazy rescale) ----------------------------
     // (CAUSAL: only tiles that cross some row's limit, a wave-uniform test)
     constexpr int KEYS = 32 * S::NT;  // keys of the tile this wave scores
@@ -259,6 +274,16 @@ __device__ __forceinline__ void compute_tile(const uint8_t* lds, uint32_t rt_off
             s[t][r] = p;
             if constexpr (!FP8) psum += p;
         }
+    if constexpr (SCALED) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const v4f x = *(const v4f*)(scales + kKeyTile + key_of_acc<F8>(t, 4 * r4, h));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][4 * r4 + i] *= x[i];
+            }
+    }
     // BF16: this lane half's share of the row sum, from the unrounded P (the
     // bf16 rounding of P below is 2^-9 relative).  FP8: the full row sum of
     // the e4m3-rounded P that the PV MFMAs consume, taken by an MFMA below.
