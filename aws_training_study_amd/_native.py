@@ -17,7 +17,7 @@ LIB_NAME = "libpcp_attention_hip.so"
 
 ABI_VERSION = 3
 # What the entry points expect of the extension's calls (csrc/fast_calls.cpp).
-FAST_CALLS_VERSION = 2
+FAST_CALLS_VERSION = 3
 
 PCPA_OK = 0
 STATUS_NAMES = {

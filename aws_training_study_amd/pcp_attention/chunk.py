@@ -61,6 +61,13 @@ class _CacheOperator:
         status = self._lib.pcpa_check_params(ctypes.byref(self._params(cfg.num_pages, 1.0, 1.0)))
         if status != _native.PCPA_OK:
             raise ValueError(f"configuration rejected by the HIP kernel: {_native.status_string(status)}")
+        self._fast = None  # the native call, made by the first one
+
+    def _native_call(self, kind: str, fn):
+        self._fast = self._native.fast_calls().make(
+            kind, bytes(self._params(self.config.num_pages, 1.0, 1.0)), self.config.kv_dtype == "fp8_e4m3fn",
+            self.config.interleave_size, self._native.function_address(fn))
+        return self._fast
 
     def _params(self, num_pages: int, k_scale: float, v_scale: float, table64: bool = False):
         return self._native.PcpaParams(num_pages=num_pages, k_scale=float(k_scale), v_scale=float(v_scale),
@@ -122,6 +129,12 @@ class ChunkCacheWriter(_CacheOperator):
 
     def __call__(self, k, v, kv_pages, block_table, lengths, *, chunk_starts=None, k_scale: float = 1.0,
                  v_scale: float = 1.0, token_scales=None) -> None:
+        call = self._fast or self._native_call("chunk_write", self._lib.pcpa_chunk_write)
+        status = call(k, v, kv_pages, block_table, lengths, chunk_starts, k_scale, v_scale, token_scales)
+        if status is not None:
+            self._native.check(status)
+            return
+        # not the common form
         import torch
 
         cfg = self.config
@@ -155,6 +168,13 @@ class CacheReader(_CacheOperator):
 
     def __call__(self, kv_pages, block_table, *, first_pos: int = 0, num_tokens: int, k_scale: float = 1.0,
                  v_scale: float = 1.0, token_scales=None):
+        call = self._fast or self._native_call("cache_read", self._lib.pcpa_cache_read)
+        result = call(kv_pages, block_table, first_pos, num_tokens, k_scale, v_scale, token_scales)
+        if type(result) is int:  # the status of a launch that failed
+            self._native.check(result)
+        if result is not None:
+            return result
+        # not the common form
         import torch
 
         cfg = self.config
@@ -240,10 +260,33 @@ class ChunkAttentionKernel(_CacheOperator):
             if ws is None and len(self._workspaces) >= 16:
                 self._workspaces.clear()
             ws = self._workspaces[key] = torch.empty(size, dtype=torch.uint8, device=device)
+            if self._fast is not None:
+                self._fast.forget()  # workspaces dropped here are dropped there too
         return ws
+
+    def _attention_call(self):
+        import weakref
+
+        import torch
+
+        native, me = self._native, weakref.ref(self)  # (the call is ours: no cycle that keeps workspaces)
+        self._fast = native.fast_calls().make_attention(
+            bytes(self._params(self.config.num_pages, 1.0, 1.0)), self.config.kv_dtype == "fp8_e4m3fn",
+            self.config.interleave_size, native.function_address(self._lib.pcpa_chunk_attention),
+            native.function_address(self._lib.pcpa_chunk_workspace_bytes),
+            lambda size, index, stream: me()._workspace(size, torch.device("cuda", index), stream))
+        return self._fast
 
     def __call__(self, q, kv_pages, block_table, lengths, *, chunk_starts=None, k_scale: float = 1.0,
                  v_scale: float = 1.0, token_scales=None, out=None, return_lse: bool = False, workspace=None):
+        call = self._fast or self._attention_call()
+        result = call(q, kv_pages, block_table, lengths, chunk_starts, k_scale, v_scale, token_scales, out, return_lse,
+                      workspace)
+        if type(result) is int:  # the status of a launch that failed
+            self._native.check(result)
+        if result is not None:
+            return result
+        # not the common form
         import torch
 
         cfg = self.config
@@ -320,9 +363,20 @@ class ChunkStep:
     def prepare(self, q, k, v, kv_pages, block_table, lengths, *, chunk_starts=None, q_weight=None, k_weight=None,
                 k_scale: float = 1.0, v_scale: float = 1.0, token_scales=None, q_out=None):
         """The first launch alone: K and V in their pages, the rotated Q returned."""
+        cfg, op, rotation = self.config, self.attention, self.rotation
+        turns = rotation._turns.get(getattr(q, "device", None))
+        if turns is not None:
+            call = rotation._fast.get("chunk_prepare") or rotation._native_call("chunk_prepare",
+                                                                                op._lib.pcpa_chunk_prepare)
+            result = call(q, k, v, kv_pages, block_table, lengths, chunk_starts, q_weight, k_weight, k_scale, v_scale,
+                          token_scales, q_out, turns)
+            if type(result) is int:  # the status of a launch that failed
+                op._native.check(result)
+            if result is not None:
+                return result
+        # not the common form
         import torch
 
-        cfg, op = self.config, self.attention
         native = op._native
         _rows("q", q, cfg.num_q_heads, cfg.head_dim, None)
         device, n = q.device, q.shape[0]

@@ -190,6 +190,16 @@ class QueryKeyRotation:
             q_dtype=_native.DTYPE_BF16, kv_dtype=_KV_DTYPE_CODES[cfg.kv_dtype], out_dtype=_native.DTYPE_BF16,
             softmax_scale=cfg.softmax_scale, k_scale=1.0, v_scale=1.0, flags=0)
         self._turns = {}  # per device: revolutions per position of every pair
+        self._fast = {}   # the native calls, made by the first ones
+
+    def _native_call(self, kind: str, fn):
+        native, rotary = self._native, self.rotary
+        static = native.PcpaRotary(rotary.rotary_dim, int(rotary.pairs == "interleaved"), native.DTYPE_BF16,
+                                   rotary.amplitude, self.norm_eps, None, None, None)
+        call = self._fast[kind] = native.fast_calls().make_rotation(
+            kind, bytes(self._params), self.config.kv_dtype == "fp8_e4m3fn", self.config.interleave_size,
+            native.function_address(fn), bytes(static))
+        return call
 
     def turns(self, device):
         """Revolutions per position of every pair, float64 on ``device`` (made once per device)."""
@@ -220,6 +230,15 @@ class QueryKeyRotation:
 
     def __call__(self, q, k, *, positions=None, lengths=None, chunk_starts=None, q_weight=None, k_weight=None,
                  q_out=None, k_out=None):
+        turns = self._turns.get(getattr(q, "device", None))
+        if turns is not None:
+            call = self._fast.get("rotate") or self._native_call("rotate", self._lib.pcpa_rotate)
+            result = call(q, k, positions, lengths, chunk_starts, q_weight, k_weight, q_out, k_out, turns)
+            if type(result) is int:  # the status of a launch that failed
+                self._native.check(result)
+            if result is not None:
+                return result
+        # not the common form
         import torch
 
         cfg, native = self.config, self._native
@@ -262,6 +281,15 @@ class QueryKeyRotation:
         return q_out, k_out
 
     def prefill(self, q, k, v, *, first_pos: int, q_weight=None, k_weight=None):
+        turns = self._turns.get(getattr(q, "device", None))
+        if turns is not None:
+            call = self._fast.get("rotate_prefill") or self._native_call("rotate_prefill", self._lib.pcpa_rotate)
+            result = call(q, k, v, first_pos, q_weight, k_weight, turns)
+            if type(result) is int:  # the status of a launch that failed
+                self._native.check(result)
+            if result is not None:
+                return result
+        # not the common form
         import torch
 
         cfg, native = self.config, self._native
