@@ -24,7 +24,6 @@ struct SequencePlan {
 struct AttendArgs {
     Desc chunk;
     Pages pages;
-    cache::FastDiv div_pcp, div_block;
     const uint8_t* q;
     const uint8_t* pool;
     const float* token_scales;
@@ -95,7 +94,31 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) work += __shfl_xor(work, off);
     const int64_t share = (work * heads + a.slots - 1) / a.slots;
-    const int range = (int)max(share, (int64_t)a.min_range);
+    int range = (int)max(share, (int64_t)a.min_range);
+    // Each sequence's last range is a shorter one, so that ranges of the fair
+    // share are more than the GPU holds at once, and the few left over would run
+    // after all others: longer ranges, until all run together.  (64 sequences of
+    // 512 to 8192 tokens, 2 heads: NEWFIG.)
+    for (int tries = 0; tries < 6; ++tries) {
+        int64_t count = 0, least = 0;
+        for (int base = 0; base < a.chunk.batch; base += 64) {
+            if (base == 0) {
+                tiles = first_tiles;
+                walk = first_walk;
+            } else {
+                sequence(base, span, length, tiles, walk);
+            }
+            count += (int64_t)tiles * ((walk + range - 1) / range);
+            least += tiles;
+        }
+#pragma unroll
+        for (int off = 32; off >= 1; off >>= 1) {
+            count += __shfl_xor(count, off);
+            least += __shfl_xor(least, off);
+        }
+        if (count * heads <= a.slots || least * heads >= a.slots) break;
+        range = (int)min((int64_t)range + max((int64_t)1, range * (count * heads - a.slots) / a.slots), (int64_t)1 << 30);
+    }
     int before = 0;
     for (int base = 0; base < a.chunk.batch; base += 64) {
         if (base == 0) {
@@ -288,11 +311,11 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
         FewStep<S> s{0, 0, 0, -1, 0, u};
         for (; s.u < steps; s.u += S::WAVES) {
             const uint32_t tile = it.begin + s.u / S::SUB;
-            const uint32_t lt = cache::div(tile, a.div_pcp);
+            const uint32_t lt = div(tile, a.pages.div_pcp);
             const int rank = tile - lt * a.pages.pcp;
             const int local = lt * kTileKeys + (s.u % S::SUB) * S::KEYS;
             const int n = min(owned(most_rounds, most_rest, rank) - local, S::KEYS);
-            const uint32_t blk = cache::div(local, a.div_block);
+            const uint32_t blk = div(local, a.pages.div_block);
             if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
             const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
             if ((unsigned)page >= (unsigned)a.pages.num_pages) continue;
@@ -718,10 +741,10 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     auto tile_from = [&](int i) {
         ManyTile t{i, -1, 0, 0, 0, 0};
         for (; t.i < end; ++t.i) {
-            const uint32_t lt = cache::div((uint32_t)t.i, a.div_pcp);
+            const uint32_t lt = div((uint32_t)t.i, a.pages.div_pcp);
             const int rank = t.i - lt * a.pages.pcp, local = lt * kKeyTile;
             const int n = min(owned(most_rounds, most_rest, rank) - local, kKeyTile);
-            const uint32_t blk = cache::div((uint32_t)local, a.div_block);
+            const uint32_t blk = div((uint32_t)local, a.pages.div_block);
             if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
             const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
             if ((unsigned)page >= (unsigned)a.pages.num_pages) continue;
@@ -922,84 +945,133 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
 
 // ---- ranges of one walk ----------------------------------------------------------
 
-// One workgroup per (row, Q head): the partial results of the ranges of the
-// row's walk, weighted by their sums.  D / 4 threads take a partial's values,
-// THREADS / (D / 4) partials at a time.
-template <int D, int THREADS>
-__global__ void __launch_bounds__(THREADS) merge_ranges_kernel(AttendArgs a) {
-    constexpr int LANES = D / 4, AT_ONCE = THREADS / LANES;
-    __shared__ v4f part[AT_ONCE][LANES];
-    __shared__ float part_ml[AT_ONCE][2];
-    const int token = blockIdx.x, head = blockIdx.y, kv = head / a.group;
-    const int b = sequence_of(a.chunk, token);
-    if (b < 0) return;
+// A row's partial results: where they are, for the row of `token` and Q head
+// `head`; false if its result is final or there is no such row.
+struct Partials {
+    int64_t first;  // row of the first range's partial result
+    int64_t step;   // rows from one range's to the next
+    int ranges;
+};
+__device__ __forceinline__ bool partials_of(const AttendArgs& a, int b, int token, int head, Partials& p) {
+    if (b < 0) return false;
     const SequencePlan plan = a.plans[b];
-    if (plan.ranges <= 1 || plan.rows <= 0) return;
+    if (plan.ranges <= 1 || plan.rows <= 0) return false;
     const Span span = span_of(a.chunk, b);
+    const int kv = head / a.group;
     const int row = (token - span.first) * a.group + (head - kv * a.group);
     const int tile = row / plan.rows;
-    const int64_t heads = a.pages.num_kv_heads, first = plan.first_item + (plan.tiles - 1 - tile) * heads + kv;
+    const int64_t heads = a.pages.num_kv_heads, item = plan.first_item + (plan.tiles - 1 - tile) * heads + kv;
     const int64_t step = plan.tiles * heads;
     // (only starts that decrease lead past the launch's items)
-    if (plan.first_item < 0 || tile >= plan.tiles || first + (plan.ranges - 1) * step >= a.max_items) return;
-    const int at = threadIdx.x / LANES, c = threadIdx.x % LANES;
-    float top = -INFINITY, total = 0.f;
-    v4f acc{0.f, 0.f, 0.f, 0.f};
-    constexpr int UNROLL = 4;
-    for (int s0 = at; s0 < plan.ranges; s0 += AT_ONCE * UNROLL) {
-        float ls[UNROLL];
-        v4f x[UNROLL];
+    if (plan.first_item < 0 || tile >= plan.tiles || item + (plan.ranges - 1) * step >= a.max_items) return false;
+    p = Partials{item * plan.rows + row % plan.rows, step * plan.rows, plan.ranges};
+    return true;
+}
+
+// The running merge of partial results: weights 2^(log2 sum - top).
+struct Merged {
+    float top, total;
+    v4f acc;
+    __device__ __forceinline__ void add(float log2sum, const v4f& x) {
+        if (log2sum == -INFINITY) return;  // nothing seen in it
+        const float next = fmaxf(top, log2sum);
+        const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+        const float weight = __builtin_amdgcn_exp2f(log2sum - next);
+        total = fmaf(total, keep, weight);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int s = s0 + u * AT_ONCE;
-            const int64_t prow = (first + min(s, plan.ranges - 1) * step) * plan.rows + row % plan.rows;
-            ls[u] = s < plan.ranges ? a.part_lse[prow] : -INFINITY;
-            x[u] = *(const v4f*)(a.part_o + prow * D + 4 * c);
-        }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            if (ls[u] == -INFINITY) continue;  // nothing seen in it, or past the last range
-            const float next = fmaxf(top, ls[u]);
-            const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
-            const float weight = __builtin_amdgcn_exp2f(ls[u] - next);
-            total = fmaf(total, keep, weight);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] = fmaf(acc[k], keep, weight * x[u][k]);
-            top = next;
-        }
+        for (int k = 0; k < 4; ++k) acc[k] = fmaf(acc[k], keep, weight * x[k]);
+        top = next;
     }
-    part[at][c] = acc;
-    if (c == 0) {
-        part_ml[at][0] = top;
-        part_ml[at][1] = total;
-    }
-    __syncthreads();
-    if (at != 0) return;
-    top = part_ml[0][0];
-#pragma unroll
-    for (int p = 1; p < AT_ONCE; ++p) top = fmaxf(top, part_ml[p][0]);
-    total = 0.f;
-    acc = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int p = 0; p < AT_ONCE; ++p) {
-        if (part_ml[p][1] == 0.f) continue;  // nothing seen (a NaN is not nothing)
-        const float weight = __builtin_amdgcn_exp2f(part_ml[p][0] - top);
-        total = fmaf(weight, part_ml[p][1], total);
-        const v4f x = part[p][c];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] = fmaf(weight, x[k], acc[k]);
-    }
+};
+
+// Four values of a merged row to the output, and (first lane) its log-sum-exp.
+template <int D>
+__device__ __forceinline__ void store_merged(const AttendArgs& a, int64_t row, int c, float top, float total, const v4f& acc) {
     const bool empty = total == 0.f;
     const float inv = empty ? 0.f : 1.f / total;
-    const int64_t out_row = (int64_t)token * a.num_q_heads + head;
     uint32_t w[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const __bf16 lo = (__bf16)(empty ? 0.f : acc[2 * k] * inv), hi = (__bf16)(empty ? 0.f : acc[2 * k + 1] * inv);
         w[k] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
     }
-    *(v2i*)(a.out + (out_row * D + 4 * c) * 2) = v2i{(int)w[0], (int)w[1]};
-    if (a.lse && c == 0) a.lse[out_row] = empty ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+    *(v2i*)(a.out + (row * D + 4 * c) * 2) = v2i{(int)w[0], (int)w[1]};
+    if (a.lse && c == 0) a.lse[row] = empty ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+// Rows with few ranges each: D / 4 threads go through a row's partials in turn.
+// A token's Q heads are a workgroup's rows, THREADS / (D / 4) at a time.
+template <int D>
+__global__ void __launch_bounds__(256) merge_few_ranges_kernel(AttendArgs a) {
+    constexpr int LANES = D / 4, AT_ONCE = 256 / LANES, UNROLL = 4;
+    const int token = blockIdx.x, b = sequence_of(a.chunk, token);
+    const int c = threadIdx.x % LANES;
+    for (int head = blockIdx.y * AT_ONCE + threadIdx.x / LANES; head < a.num_q_heads; head += gridDim.y * AT_ONCE) {
+        Partials p;
+        if (!partials_of(a, b, token, head, p)) continue;
+        Merged r{-INFINITY, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
+        for (int s0 = 0; s0 < p.ranges; s0 += UNROLL) {
+            float ls[UNROLL];
+            v4f x[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const int64_t row = p.first + min(s0 + u, p.ranges - 1) * p.step;
+                ls[u] = a.part_lse[row];
+                x[u] = *(const v4f*)(a.part_o + row * D + 4 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) r.add(s0 + u < p.ranges ? ls[u] : -INFINITY, x[u]);
+        }
+        store_merged<D>(a, (int64_t)token * a.num_q_heads + head, c, r.top, r.total, r.acc);
+    }
+}
+
+// Rows with many ranges: a workgroup of 16 waves per (row, Q head), 1024 / (D / 4)
+// partials at a time, which meet in LDS.
+template <int D>
+__global__ void __launch_bounds__(1024) merge_many_ranges_kernel(AttendArgs a) {
+    constexpr int LANES = D / 4, AT_ONCE = 1024 / LANES, UNROLL = 4;
+    __shared__ v4f part[AT_ONCE][LANES];
+    __shared__ float part_ml[AT_ONCE][2];
+    const int token = blockIdx.x, head = blockIdx.y;
+    const int b = sequence_of(a.chunk, token);
+    Partials p;
+    if (!partials_of(a, b, token, head, p)) return;
+    const int at = threadIdx.x / LANES, c = threadIdx.x % LANES;
+    Merged r{-INFINITY, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
+    for (int s0 = at; s0 < p.ranges; s0 += AT_ONCE * UNROLL) {
+        float ls[UNROLL];
+        v4f x[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int64_t row = p.first + min(s0 + u * AT_ONCE, p.ranges - 1) * p.step;
+            ls[u] = a.part_lse[row];
+            x[u] = *(const v4f*)(a.part_o + row * D + 4 * c);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) r.add(s0 + u * AT_ONCE < p.ranges ? ls[u] : -INFINITY, x[u]);
+    }
+    part[at][c] = r.acc;
+    if (c == 0) {
+        part_ml[at][0] = r.top;
+        part_ml[at][1] = r.total;
+    }
+    __syncthreads();
+    if (at != 0) return;
+    const int n = min(p.ranges, AT_ONCE);
+    float top = part_ml[0][0];
+    for (int i = 1; i < n; ++i) top = fmaxf(top, part_ml[i][0]);
+    float total = 0.f;
+    v4f acc{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; ++i) {
+        if (part_ml[i][1] == 0.f) continue;  // nothing seen (a NaN is not nothing)
+        const float weight = __builtin_amdgcn_exp2f(part_ml[i][0] - top);
+        total = fmaf(weight, part_ml[i][1], total);
+        const v4f x = part[i][c];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = fmaf(weight, x[k], acc[k]);
+    }
+    store_merged<D>(a, (int64_t)token * a.num_q_heads + head, c, top, total, acc);
 }
 
 }  // namespace chunk

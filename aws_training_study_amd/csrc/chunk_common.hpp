@@ -2,6 +2,7 @@
 // which sequence and position a row has, and where a position's page is.
 #pragma once
 
+#include "cache_kernels.hpp"
 #include "common.hpp"
 #include "paging_kernels.hpp"
 
@@ -45,6 +46,20 @@ __device__ __forceinline__ int sequence_of(const Desc& c, int token) {
     return token >= s.first && token < s.first + s.count ? b : -1;
 }
 
+// floor(n / d) for 0 <= n < 2^31 in three instructions: m = floor(2^(31 + l) / d)
+// + 1 with 2^l >= d fits 32 bits and is off from 2^(31 + l) / d by at most one,
+// which n < 2^31 does not carry over a whole number.
+struct Div {
+    uint32_t m;
+    uint32_t shift;
+};
+inline Div make_div(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return Div{(uint32_t)((1ull << (31 + l)) / d + 1), 31 + l};
+}
+__device__ __forceinline__ uint32_t div(uint32_t n, const Div& d) { return (uint32_t)(((uint64_t)n * d.m) >> d.shift); }
+
 struct Pages {
     const int32_t* table;  // [batch, pcp, max_local_blocks], int32 or int64 as dword pairs
     int32_t table_shift;
@@ -54,6 +69,7 @@ struct Pages {
     int32_t pcp;
     int32_t interleave;
     int32_t num_kv_heads;
+    Div div_interleave, div_pcp, div_block;
     int32_t capacity;      // positions of a sequence's cache: pcp * max_local_blocks * block_size
     int64_t page_stride;   // bytes of a page
     int64_t head_stride;   // bytes of one head's K (or V) of a page
@@ -76,10 +92,10 @@ struct Place {
 };
 __device__ __forceinline__ Place place_of(const Pages& p, int64_t first, int64_t pos) {
     if (pos < 0 || pos >= p.capacity) return Place{-1, 0};
-    const uint32_t at = (uint32_t)pos, il = p.interleave, pcp = p.pcp;
-    const uint32_t c = at / il, round = c / pcp, rank = c - round * pcp;
-    const uint32_t local = round * il + (at - c * il);
-    const uint32_t blk = local / (uint32_t)p.block_size;
+    const uint32_t at = (uint32_t)pos;
+    const uint32_t c = div(at, p.div_interleave), round = div(c, p.div_pcp), rank = c - round * p.pcp;
+    const uint32_t local = round * p.interleave + (at - c * p.interleave);
+    const uint32_t blk = div(local, p.div_block);
     // (the last round of a bucket that is no whole number of rounds)
     if (blk >= (uint32_t)p.max_local_blocks) return Place{-1, 0};
     return Place{page_at(p, first, (int)(rank * p.max_local_blocks + blk)), (int)(local - blk * p.block_size)};

@@ -9,6 +9,8 @@ namespace pcpa {
 namespace chunk {
 namespace {
 
+constexpr int kCUs = 256;  // MI355X
+
 // The parameters and the chunk, without the pointers that the kernels read.
 int32_t check_chunk(const pcpa_params* p, const pcpa_chunk* c) {
     const int32_t st = pcpa_check_params(p);
@@ -51,6 +53,9 @@ Pages pages_of(const pcpa_params* p, int32_t interleave, const void* block_table
     g.pcp = p->pcp_size;
     g.interleave = interleave;
     g.num_kv_heads = p->num_kv_heads;
+    g.div_interleave = make_div((uint32_t)interleave);
+    g.div_pcp = make_div((uint32_t)p->pcp_size);
+    g.div_block = make_div((uint32_t)p->block_size);
     g.capacity = (int32_t)((int64_t)p->pcp_size * p->max_local_blocks * p->block_size);
     g.head_stride = (int64_t)p->block_size * p->head_dim * es;
     g.page_stride = 2 * (int64_t)p->num_kv_heads * g.head_stride;
@@ -70,7 +75,7 @@ int32_t check_rotary(const pcpa_params* p, const pcpa_rotary* r) {
     if (!isfinite(r->amplitude) || !isfinite(r->norm_eps) || r->norm_eps < 0.f) return PCPA_ERR_BAD_SCALE;
     const bool f32 = r->weight_dtype == PCPA_DTYPE_FP32;
     if (!f32 && r->weight_dtype != PCPA_DTYPE_BF16) return PCPA_ERR_BAD_DTYPE;
-    if (((uintptr_t)r->q_weight | (uintptr_t)r->k_weight) & (f32 ? 3u : 1u)) return PCPA_ERR_MISALIGNED;
+    if (((uintptr_t)r->q_weight | (uintptr_t)r->k_weight) & (f32 ? 15u : 7u)) return PCPA_ERR_MISALIGNED;
     if ((uintptr_t)r->turns & 7u) return PCPA_ERR_MISALIGNED;
     return PCPA_OK;
 }
@@ -86,30 +91,47 @@ void set_rotary(TokenArgs& a, const pcpa_rotary* r) {
     a.weight_f32 = r->weight_dtype == PCPA_DTYPE_FP32;
 }
 
-template <bool ROTATE, bool PAGES, bool FP8>
+template <bool ROTATE, bool PAGES, bool FP8, int NG>
 const void* token_kernel_for(int head_dim) {
-    return head_dim == 64    ? (const void*)token_kernel<64, ROTATE, PAGES, FP8>
-           : head_dim == 128 ? (const void*)token_kernel<128, ROTATE, PAGES, FP8>
-                             : (const void*)token_kernel<256, ROTATE, PAGES, FP8>;
+    return head_dim == 64    ? (const void*)token_kernel<64, ROTATE, PAGES, FP8, NG>
+           : head_dim == 128 ? (const void*)token_kernel<128, ROTATE, PAGES, FP8, NG>
+                             : (const void*)token_kernel<256, ROTATE, PAGES, FP8, NG>;
 }
 
-constexpr int kWavesInFlight = 256 * 16;
+struct ReadKernel {
+    const void* fn;
+    int tokens;
+};
+template <bool FP8>
+ReadKernel read_kernel_for(int d) {
+    return d == 64    ? ReadKernel{(const void*)cache_read_kernel<64, FP8>, read_tokens<64>()}
+           : d == 128 ? ReadKernel{(const void*)cache_read_kernel<128, FP8>, read_tokens<128>()}
+                      : ReadKernel{(const void*)cache_read_kernel<256, FP8>, read_tokens<256>()};
+}
 
-int32_t launch_tokens(const void* fn, TokenArgs& a, const pcpa_params* p, hipStream_t stream) {
+template <bool ROTATE, bool PAGES, bool FP8>
+int32_t launch_tokens(TokenArgs& a, const pcpa_params* p, hipStream_t stream) {
     a.num_q_heads = p->num_q_heads;
     a.num_kv_heads = p->num_kv_heads;
-    a.rows_per_token = (a.q.data ? p->num_q_heads : 0) + (a.k.data ? p->num_kv_heads : 0) +
-                       (a.v.data ? p->num_kv_heads : 0);
-    const int rows = 64 / (p->head_dim / 8), groups = (a.rows_per_token + rows - 1) / rows;
-    // a wave takes several groups of a token's rows once there are enough
-    // waves for the GPU without
-    const int64_t each = (int64_t)a.chunk.num_tokens * groups / kWavesInFlight;
-    a.groups_per_wave = (int)(each < 1 ? 1 : each > groups ? groups : each);
-    a.waves_per_token = (groups + a.groups_per_wave - 1) / a.groups_per_wave;
-    const int64_t waves = (int64_t)a.chunk.num_tokens * a.waves_per_token, per = kTokenThreads / 64;
-    const int64_t blocks = (waves + per - 1) / per;
+    const int rows = token_rows(p->head_dim), kv_groups = (p->num_kv_heads + rows - 1) / rows;
+    const int q_groups = a.q.data ? (p->num_q_heads + rows - 1) / rows : 0, kinds = (a.k.data ? 1 : 0) + (a.v.data ? 1 : 0);
+    const int64_t n = a.chunk.num_tokens;
+    // four groups a wave once that fills half the GPU's 32 waves a CU
+    const int ng = n * (q_groups + kinds * kv_groups) >= 4ll * 16 * kCUs ? 4 : 1;
+    const int64_t q_parts = (q_groups + ng - 1) / ng, blocks_of_tokens = (n + ng - 1) / ng;
+    const int64_t q_waves = n * q_parts, kv_waves = blocks_of_tokens * kv_groups;
+    const int64_t waves = q_waves + kinds * kv_waves, per = kTokenThreads / 64, blocks = (waves + per - 1) / per;
     if (waves > INT32_MAX - per) return PCPA_ERR_TOO_LARGE;
+    a.waves = (int32_t)waves;
+    a.q_waves = (int32_t)q_waves;
+    a.q_parts = (int32_t)q_parts;
+    a.kv_waves = (int32_t)kv_waves;
+    a.token_blocks = (int32_t)blocks_of_tokens;
+    a.div_q_parts = make_div((uint32_t)(q_parts > 0 ? q_parts : 1));
+    a.div_token_blocks = make_div((uint32_t)blocks_of_tokens);
     void* args[] = {&a};
+    const void* const fn = ng == 4 ? token_kernel_for<ROTATE, PAGES, FP8, 4>(p->head_dim)
+                                   : token_kernel_for<ROTATE, PAGES, FP8, 1>(p->head_dim);
     return hipLaunchKernel(fn, dim3((unsigned)blocks), dim3(kTokenThreads), args, 0, stream) == hipSuccess
                ? PCPA_OK
                : PCPA_ERR_LAUNCH;
@@ -143,10 +165,8 @@ int32_t write_chunk(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary
     a.k_scale = p->k_scale;
     a.v_scale = p->v_scale;
     const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
-    const int d = p->head_dim;
-    const void* const fn = r ? (fp8 ? token_kernel_for<true, true, true>(d) : token_kernel_for<true, true, false>(d))
-                             : (fp8 ? token_kernel_for<false, true, true>(d) : token_kernel_for<false, true, false>(d));
-    return launch_tokens(fn, a, p, stream);
+    return r ? (fp8 ? launch_tokens<true, true, true>(a, p, stream) : launch_tokens<true, true, false>(a, p, stream))
+             : (fp8 ? launch_tokens<false, true, true>(a, p, stream) : launch_tokens<false, true, false>(a, p, stream));
 }
 
 // ---- attention ---------------------------------------------------------------
@@ -182,7 +202,6 @@ AttendKernel many_kernel_for(int d, bool scaled) {
     return d == 64 ? many_kernel<64, FP8>(scaled) : d == 128 ? many_kernel<128, FP8>(scaled) : many_kernel<256, FP8>(scaled);
 }
 
-constexpr int kCUs = 256;  // MI355X
 // A range of a walk has at least this many tiles (64 keys each).
 constexpr int kMinRange = 8;
 
@@ -219,8 +238,8 @@ AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = 
 }
 
 template <int D>
-const void* merge_kernel_for(bool wide) {
-    return wide ? (const void*)merge_ranges_kernel<D, 1024> : (const void*)merge_ranges_kernel<D, 256>;
+const void* merge_kernel_for(bool many) {
+    return many ? (const void*)merge_many_ranges_kernel<D> : (const void*)merge_few_ranges_kernel<D>;
 }
 
 int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const void* kv_pages,
@@ -239,8 +258,6 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     AttendArgs a{};
     a.chunk = desc_of(c);
     a.pages = pages_of(p, c->interleave, block_table);
-    a.div_pcp = cache::make_fastdiv((uint32_t)p->pcp_size);
-    a.div_block = cache::make_fastdiv((uint32_t)p->block_size);
     a.q = (const uint8_t*)q;
     a.pool = (const uint8_t*)kv_pages;
     a.token_scales = token_scales;
@@ -262,15 +279,16 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     if (hipLaunchKernel(w.kernel.fn, dim3((unsigned)w.items), dim3(w.kernel.threads), args, 0, stream) != hipSuccess)
         return PCPA_ERR_LAUNCH;
     if (!w.ranges) return PCPA_OK;
-    // few rows: many ranges each, taken by 16 waves
-    const bool wide = (int64_t)c->num_tokens * p->num_q_heads <= kCUs;
-    const void* const merge = p->head_dim == 64    ? merge_kernel_for<64>(wide)
-                              : p->head_dim == 128 ? merge_kernel_for<128>(wide)
-                                                   : merge_kernel_for<256>(wide);
-    return hipLaunchKernel(merge, dim3(c->num_tokens, p->num_q_heads), dim3(wide ? 1024 : 256), args, 0, stream) ==
-                   hipSuccess
-               ? PCPA_OK
-               : PCPA_ERR_LAUNCH;
+    // Few rows have many ranges each: 16 waves to a row, as long as the GPU has
+    // room for all rows at once
+    const bool many = (int64_t)c->num_tokens * p->num_q_heads <= 2 * kCUs;
+    const void* const merge = p->head_dim == 64    ? merge_kernel_for<64>(many)
+                              : p->head_dim == 128 ? merge_kernel_for<128>(many)
+                                                   : merge_kernel_for<256>(many);
+    const int at_once = 256 / (p->head_dim / 4);
+    const dim3 grid(c->num_tokens, many ? p->num_q_heads : (p->num_q_heads + at_once - 1) / at_once);
+    return hipLaunchKernel(merge, grid, dim3(many ? 1024 : 256), args, 0, stream) == hipSuccess ? PCPA_OK
+                                                                                               : PCPA_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -305,8 +323,7 @@ int32_t pcpa_rotate(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary
     if (c->num_tokens == 0) return PCPA_OK;
     TokenArgs a{};
     a.chunk = desc_of(c);
-    a.pages.pcp = p->pcp_size;
-    a.pages.interleave = c->interleave;
+    a.pages = pages_of(p, c->interleave, nullptr);
     a.q = rows_in(q);
     a.k = rows_in(k);
     a.q_out = rows_out(q_out);
@@ -321,7 +338,7 @@ int32_t pcpa_rotate(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary
     a.positions = positions;
     a.first_pos = first_pos;
     set_rotary(a, r);
-    return launch_tokens(token_kernel_for<true, false, false>(p->head_dim), a, p, (hipStream_t)stream);
+    return launch_tokens<true, false, false>(a, p, (hipStream_t)stream);
 }
 
 int32_t pcpa_chunk_write(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rows* k, const pcpa_rows* v,
@@ -361,16 +378,11 @@ int32_t pcpa_cache_read(const pcpa_params* p, int32_t interleave, int64_t first_
     a.k_scale = p->k_scale;
     a.v_scale = p->v_scale;
     const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
-    const void* const fn = p->head_dim == 64    ? (fp8 ? (const void*)cache_read_kernel<64, true>
-                                                       : (const void*)cache_read_kernel<64, false>)
-                           : p->head_dim == 128 ? (fp8 ? (const void*)cache_read_kernel<128, true>
-                                                       : (const void*)cache_read_kernel<128, false>)
-                                                : (fp8 ? (const void*)cache_read_kernel<256, true>
-                                                       : (const void*)cache_read_kernel<256, false>);
-    const int64_t blocks = ((int64_t)num_tokens * (p->head_dim / 8) + kTokenThreads - 1) / kTokenThreads;
-    if (blocks > INT32_MAX || p->num_kv_heads > 65535) return PCPA_ERR_TOO_LARGE;
+    const ReadKernel kernel = fp8 ? read_kernel_for<true>(p->head_dim) : read_kernel_for<false>(p->head_dim);
+    const int64_t blocks = ((int64_t)num_tokens + kernel.tokens - 1) / kernel.tokens;
+    if (p->num_kv_heads > 65535) return PCPA_ERR_TOO_LARGE;
     void* args[] = {&a};
-    return hipLaunchKernel(fn, dim3((unsigned)blocks, p->num_kv_heads, 2), dim3(kTokenThreads), args, 0,
+    return hipLaunchKernel(kernel.fn, dim3((unsigned)blocks, p->num_kv_heads, 2), dim3(kTokenThreads), args, 0,
                            (hipStream_t)stream) == hipSuccess
                ? PCPA_OK
                : PCPA_ERR_LAUNCH;

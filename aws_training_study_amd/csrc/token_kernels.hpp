@@ -29,8 +29,11 @@ struct TokenArgs {
     RowsIn q, k, v;
     RowsOut q_out, k_out, v_out;
     int32_t num_q_heads, num_kv_heads;
-    int32_t rows_per_token;  // heads of q, k and v that are there
-    int32_t waves_per_token, groups_per_wave;
+    // waves: q_waves of Q (q_parts a token, NG groups each), then kv_waves of K and
+    // as many of V (each group of heads over token_blocks runs of NG tokens)
+    int32_t q_waves, q_parts, kv_waves, token_blocks;
+    int32_t waves;        // all of them: a workgroup's last may be of none
+    Div div_q_parts, div_token_blocks;
     int32_t striped;      // q_out is [pcp, Hq, local_q, D]
     int32_t local_q;
     int32_t position_kind;
@@ -49,10 +52,6 @@ struct TokenArgs {
     float k_scale, v_scale;
 };
 
-__device__ __forceinline__ float weight_at(const uint8_t* w, int d, int f32) {
-    return f32 ? ((const float*)w)[d] : bf16_bits_to_f32(((const uint16_t*)w)[d]);
-}
-
 __device__ __forceinline__ v4i to_bf16x8(const float (&x)[8]) {
     v4i r;
 #pragma unroll
@@ -62,155 +61,325 @@ __device__ __forceinline__ v4i to_bf16x8(const float (&x)[8]) {
     }
     return r;
 }
-__device__ __forceinline__ void from_bf16x8(const v4i& r, float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = bf16_bits_to_f32((uint32_t)r[i] & 0xffffu);
-        x[2 * i + 1] = bf16_bits_to_f32((uint32_t)r[i] >> 16);
+// Sum / maximum over the LANES (8, 16 or 32) neighbouring lanes of a row:
+// exchanges within 16 lanes by DPP (quads, halves and rows mirrored once the
+// smaller groups agree), then lanes 16 apart by a row swap.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int LANES, class F>
+__device__ __forceinline__ uint32_t over_row(uint32_t x, F f) {
+    x = f(x, dpp<0xB1>(x));   // lane ^ 1
+    x = f(x, dpp<0x4E>(x));   // lane ^ 2
+    x = f(x, dpp<0x141>(x));  // half rows mirrored: lane 7 - i of 8
+    if constexpr (LANES >= 16) x = f(x, dpp<0x140>(x));  // rows mirrored: lane 15 - i of 16
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = f(r[0], r[1]);
     }
+    return x;
+}
+template <int LANES>
+__device__ __forceinline__ float sum_over_row(float x) {
+    return __uint_as_float(over_row<LANES>(__float_as_uint(x), [](uint32_t u, uint32_t v) {
+        return __float_as_uint(__uint_as_float(u) + __uint_as_float(v));
+    }));
 }
 
-// A wave takes one token and `groups_per_wave` groups of its rows (heads of Q,
-// then K, then V): a row's D values lie 8 to a lane in D / 8 neighbouring
-// lanes, 64 / (D / 8) rows at a time.  The angles of a lane's pairs depend on
-// the token and the lane alone, so they are formed once for all its rows.
+__host__ __device__ constexpr int token_rows(int d) { return 64 / (d / 8); }  // rows of a group
+
+// A group is 64 / (D / 8) heads of one token's Q, K or V, a row's D values 8 to
+// a lane in D / 8 neighbouring lanes.  A wave takes NG groups of one kind: of Q,
+// neighbouring heads of one token; of K or V, one group of heads of neighbouring
+// tokens.  Of the rotated values in the half layout a lane takes four and their
+// four partners, else eight in a row: both values of a pair are in one lane.
 //   ROTATE  norms and rotation of the q and k rows
 //   PAGES   k and v rows go into the pages (FP8: e4m3 ones), else to k_out and
 //           v_out
-// Everything is HBM bound: 2 bytes read and 1 or 2 written per value.
-template <int D, bool ROTATE, bool PAGES, bool FP8>
+// HBM bound by its bytes (2 read and 1 or 2 written per value) only as long as a
+// group costs less than about 180 vector and, as the four SIMDs share one scalar
+// unit, 45 scalar instructions, and waits are few.  So: the groups of a wave are
+// a stride apart; the rows are loaded before the tokens' places are known, which
+// take two dependent loads; sums, maxima and quotients run side by side (no
+// branch until the stores); sine and cosine are the hardware's (2^-23 off at most
+// over 2^22 even steps of a turn).  NG is 4 where that still leaves the GPU full
+// of waves, else 1: the wait is shorter (4096
+// tokens of 32 + 2 + 2 heads at D 256, normed, a quarter rotated, laid out for a
+// prefill: 31.7 us, 4.8 TB/s, where a 256 MiB copy reaches 5.5; 53.9 us when the
+// groups took 709 vector and 782 scalar instructions instead of 509 and 265).
+template <int D, bool ROTATE, bool PAGES, bool FP8, int NG>
 __global__ void __launch_bounds__(kTokenThreads) token_kernel(TokenArgs a) {
-    constexpr int LANES = D / 8, ROWS = 64 / LANES;  // lanes of a row, rows at a time
-    const int lane = threadIdx.x & 63, c = lane % LANES;
+    constexpr int LANES = D / 8, ROWS = token_rows(D);  // lanes of a row, rows of a group
+    const int lane = threadIdx.x & 63, c = lane % LANES, r = lane / LANES;
     const int wid = __builtin_amdgcn_readfirstlane((blockIdx.x * kTokenThreads + threadIdx.x) >> 6);
-    const int token = wid / a.waves_per_token, part = wid - token * a.waves_per_token;
-    if (token >= a.chunk.num_tokens) return;
 
-    // ---- the token's position and place --------------------------------------
-    int64_t pos = 0;
-    int b = 0;
-    if (a.position_kind == kOfChunk) {
-        b = sequence_of(a.chunk, token);
-        if (b < 0) return;
-        const Span s = span_of(a.chunk, b);
-        pos = (int64_t)a.chunk.lengths[b] - s.count + (token - s.first);
-    } else if (a.position_kind == kFromFirst) {
-        pos = a.first_pos + token;
+    if (wid >= a.waves) return;
+
+    // ---- the wave's groups: group i is token0 + i * dt, heads head0 + i * dh + [0, ROWS) ----
+    const bool is_q = wid < a.q_waves, is_v = !is_q && wid >= a.q_waves + a.kv_waves;
+    int token0, head0, dt;
+    if (is_q) {
+        token0 = (int)div((uint32_t)wid, a.div_q_parts);
+        head0 = (wid - token0 * a.q_parts) * (NG * ROWS);
+        dt = 0;
     } else {
-        pos = a.position_kind == kInt64 ? ((const int64_t*)a.positions)[token] : ((const int32_t*)a.positions)[token];
+        const int w = wid - a.q_waves - (is_v ? a.kv_waves : 0);
+        const int hg = (int)div((uint32_t)w, a.div_token_blocks);
+        token0 = (w - hg * a.token_blocks) * NG;
+        head0 = hg * ROWS;
+        dt = 1;
     }
-    Place at{-1, 0};
-    if constexpr (PAGES) at = place_of(a.pages, table_of(a.pages, b), pos);
+    const int dh = (1 - dt) * ROWS, heads = is_q ? a.num_q_heads : a.num_kv_heads;
+    const int tokens = dt ? min(NG, a.chunk.num_tokens - token0) : 1;
+    auto there = [&](int i) { return (dt == 0 || i < tokens) && head0 + i * dh + r < heads; };
 
-    // ---- cosines and sines of this lane's pairs ---------------------------------
-    // half layout: lane c holds values 8c .. 8c + 7, pairs i = those modulo R / 2;
-    // interleaved: pairs 4c .. 4c + 3
-    const int chunks = ROTATE ? a.rotary_dim / 8 : 0;  // lanes of a row that rotate
-    const bool turning = ROTATE && c < chunks;
-    const bool second = turning && !a.interleaved && c >= chunks / 2;
-    const int partner = lane + (second ? -chunks / 2 : chunks / 2);
-    float cosv[8], sinv[8];
-    if constexpr (ROTATE) {
+    // this lane's values of a row: [d0, d0 + 4) and [d1, d1 + 4)
+    const bool turning = ROTATE && !is_v && 8 * c < a.rotary_dim;
+    const bool apart = turning && !a.interleaved;
+    const int d0 = apart ? 4 * c : 8 * c, d1 = apart ? 4 * c + a.rotary_dim / 2 : 8 * c + 4;
+
+    // ---- the rows and the weights -----------------------------------------------------------
+    v2i raw[NG][2];
+    {
+        const RowsIn in = is_q ? a.q : is_v ? a.v : a.k;
+        const uint8_t* src = in.data + token0 * in.token_stride + head0 * in.head_stride;
+        const int64_t step = dt ? in.token_stride : dh * in.head_stride, mine = r * in.head_stride + 2 * d0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i, src += step) {
+            raw[i][0] = raw[i][1] = v2i{0, 0};
+            if (!there(i)) continue;
+            raw[i][0] = *(const v2i*)(src + mine);
+            raw[i][1] = *(const v2i*)(src + mine + 2 * (d1 - d0));
+        }
+    }
+    auto unpack = [](const v2i (&x)[2], float (&y)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int i = a.interleaved ? 4 * c + e / 2 : 8 * (second ? c - chunks / 2 : c) + e;
-            float x = 0.f, y = 0.f;
-            if (turning) {
-                const double t = (double)pos * a.turns[i];
-                const float r = (float)(t - rint(t));  // revolutions in [-1/2, 1/2]
-                sincospif(2.f * r, &y, &x);
-                x *= a.amplitude;
-                y *= a.amplitude;
-            }
-            cosv[e] = x;
-            // (a, b) -> (a cos - b sin, b cos + a sin): the sign of the partner's part
-            sinv[e] = a.interleaved ? ((e & 1) ? y : -y) : (second ? y : -y);
+            const uint32_t w = (uint32_t)x[e >> 2][(e >> 1) & 1];
+            y[e] = (e & 1) ? __uint_as_float(w & 0xffff0000u) : __uint_as_float(w << 16);
+        }
+    };
+    const uint8_t* const weight = !ROTATE || is_v ? nullptr : is_q ? a.q_weight : a.k_weight;
+    float w8[8];
+    if constexpr (ROTATE) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w8[e] = 1.f;
+        if (weight && a.weight_f32) {
+            const v4f lo = *(const v4f*)(weight + 4 * d0), hi = *(const v4f*)(weight + 4 * d1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w8[e] = e < 4 ? lo[e] : hi[e - 4];
+        } else if (weight) {
+            const v2i x[2] = {*(const v2i*)(weight + 2 * d0), *(const v2i*)(weight + 2 * d1)};
+            unpack(x, w8);
         }
     }
 
-    for (int g = 0; g < a.groups_per_wave; ++g) {
-        const int row = (part * a.groups_per_wave + g) * ROWS + lane / LANES;
-        if ((part * a.groups_per_wave + g) * ROWS >= a.rows_per_token) break;  // wave-uniform
-        // which head of q, k or v
-        const int nq = a.q.data ? a.num_q_heads : 0, nk = a.k.data ? a.num_kv_heads : 0;
-        const bool there = row < a.rows_per_token;
-        const bool is_q = there && row < nq, is_k = there && !is_q && row < nq + nk, is_v = there && !is_q && !is_k;
-        const int head = is_q ? row : is_k ? row - nq : row - nq - nk;
-        const RowsIn in = is_q ? a.q : is_k ? a.k : a.v;
-        v4i raw{0, 0, 0, 0};
-        if (there) raw = *(const v4i*)(in.data + token * in.token_stride + head * in.head_stride + c * 16);
-        float x[8];
-        from_bf16x8(raw, x);
-        if constexpr (ROTATE) {
-            const uint8_t* const w = is_q ? a.q_weight : is_k ? a.k_weight : nullptr;
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-#pragma unroll
-            for (int off = 1; off < LANES; off <<= 1) sum += __shfl_xor(sum, off);
-            if (w) {
-                const float inv = 1.f / sqrtf(sum * (1.f / D) + a.norm_eps);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * weight_at(w, 8 * c + e, a.weight_f32);
-            }
-            float y[8];  // the other value of each pair
-            if (a.interleaved) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[e ^ 1];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = __shfl(x[e], partner);
-            }
-            if (turning && (is_q || is_k)) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], cosv[e], y[e] * sinv[e]);
-            }
-            // v's rows and those without norm and rotation keep their bits
-            if (is_q || is_k) raw = to_bf16x8(x);
-        }
-        if (is_q || (!PAGES && there)) {
-            uint8_t* dst;
-            if (is_q && a.striped) {
-                const int il = a.pages.interleave, pcp = a.pages.pcp;
-                const int ch = token / il, round = ch / pcp, rank = ch - round * pcp;
-                const int local = round * il + (token - ch * il);
-                dst = a.q_out.data + (((int64_t)rank * a.num_q_heads + head) * a.local_q + local) * D * 2;
-            } else {
-                const RowsOut out = is_q ? a.q_out : is_k ? a.k_out : a.v_out;
-                dst = out.data + token * out.token_stride + head * out.head_stride;
-            }
-            *(v4i*)(dst + c * 16) = raw;
-        }
-        if constexpr (PAGES) {
-            // (the row's bf16 values are what is quantised, rotated or not)
-            const bool stored = (is_k || is_v) && at.page >= 0;
-            const int64_t offset = at.page * a.pages.page_stride +
-                                   (int64_t)(is_v ? a.num_kv_heads + head : head) * a.pages.head_stride +
-                                   (int64_t)at.slot * D * (FP8 ? 1 : 2) + c * (FP8 ? 8 : 16);
-            if constexpr (FP8) {
-                from_bf16x8(raw, x);
-                float scale = is_v ? a.v_scale : a.k_scale;
-                if (a.token_scales) {
-                    uint32_t m = 0;  // the largest finite magnitude's bits
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
-                        m = u < 0x7f800000u ? max(m, u) : m;
+    // ---- the tokens' positions and places, token i in lane i --------------------------------
+    int64_t pos = 0;
+    Place at{-1, 0};
+    bool live = lane < tokens;
+    {
+        const int token = token0 + min(lane, tokens - 1);
+        int b = 0;
+        if (a.position_kind == kOfChunk) {
+            Span s{0, 0};
+            int64_t length = 0;
+            if (!a.chunk.starts) {
+                b = token / a.chunk.each;
+                s = span_of(a.chunk, b);
+                length = a.chunk.lengths[b];
+            } else if (a.chunk.batch <= 64) {
+                // the sequences' starts and lengths, one to a lane, in one wait
+                const bool has = lane < a.chunk.batch;
+                const Span mine = has ? span_of(a.chunk, lane) : Span{0, 0};
+                const int len = has ? a.chunk.lengths[lane] : 0;
+                const int end = has ? mine.first + mine.count : INT32_MAX;
+                b = -1;
+                for (int i = 0; i < tokens; ++i) {
+                    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= token0 + i));
+                    if (n >= a.chunk.batch) continue;
+                    const Span of{__builtin_amdgcn_readlane(mine.first, n), __builtin_amdgcn_readlane(mine.count, n)};
+                    const int of_length = __builtin_amdgcn_readlane(len, n);
+                    if (lane == i && token0 + i >= of.first && token0 + i < of.first + of.count) {
+                        b = n;
+                        s = of;
+                        length = of_length;
                     }
+                }
+            } else {
+                b = -1;
+                for (int i = 0; i < tokens; ++i) {
+                    const int found = sequence_of(a.chunk, token0 + i);
+                    b = lane == i ? found : b;
+                }
+                if (live && b >= 0) {
+                    s = span_of(a.chunk, b);
+                    length = a.chunk.lengths[b];
+                }
+            }
+            live = live && b >= 0;
+            pos = length - s.count + (token - s.first);
+        } else if (a.position_kind == kFromFirst) {
+            pos = a.first_pos + token;
+        } else {
+            pos = a.position_kind == kInt64 ? ((const int64_t*)a.positions)[token] : ((const int32_t*)a.positions)[token];
+        }
+        if (PAGES && !is_q && live) at = place_of(a.pages, table_of(a.pages, b), pos);
+    }
+    const uint64_t live_mask = __builtin_amdgcn_ballot_w64(live);
+    if (!live_mask) return;
+
+    // ---- norms and rotation ---------------------------------------------------------------------
+    if (ROTATE && !is_v) {
+        float cosv[4] = {1.f, 1.f, 1.f, 1.f}, sinv[4] = {};
 #pragma unroll
-                    for (int off = 1; off < LANES; off <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off));
-                    scale = fmaxf(__uint_as_float(m) / kFp8Max, kScaleFloor);
-                    if (stored && c == 0)
-                        a.token_scales[((int64_t)at.page * 2 * a.num_kv_heads + (is_v ? a.num_kv_heads : 0) + head) *
-                                           a.pages.block_size + at.slot] = scale;
+        for (int i = 0; i < NG; ++i) {
+            if (a.rotary_dim > 0 && (i == 0 || dt)) {
+                const int64_t p = ((int64_t)__builtin_amdgcn_readlane((int)(pos >> 32), i) << 32) |
+                                  (uint32_t)__builtin_amdgcn_readlane((int)pos, i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double t = (double)p * a.turns[turning ? 4 * c + e : 0];
+                    const float x = (float)(t - rint(t));  // revolutions in [-1/2, 1/2]
+                    sinv[e] = __builtin_amdgcn_sinf(x) * a.amplitude;
+                    cosv[e] = __builtin_amdgcn_cosf(x) * a.amplitude;
+                }
+            }
+            float x[8];
+            unpack(raw[i], x);
+            if (weight) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+                sum = sum_over_row<LANES>(sum);
+                const float inv = __builtin_amdgcn_rsqf(sum * (1.f / D) + a.norm_eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] *= inv * w8[e];
+            }
+            if (turning) {
+                // half layout: pairs (e, e + 4); interleaved: (2 e, 2 e + 1)
+                if (a.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = x[2 * e], v = x[2 * e + 1];
+                        x[2 * e] = fmaf(u, cosv[e], -v * sinv[e]);
+                        x[2 * e + 1] = fmaf(v, cosv[e], u * sinv[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = x[e], v = x[e + 4];
+                        x[e] = fmaf(u, cosv[e], -v * sinv[e]);
+                        x[e + 4] = fmaf(v, cosv[e], u * sinv[e]);
+                    }
+                }
+            }
+            const v4i z = to_bf16x8(x);
+            raw[i][0] = v2i{z[0], z[1]};
+            raw[i][1] = v2i{z[2], z[3]};
+        }
+    }
+
+    // ---- rows of q, and of k and v without pages ---------------------------------------------------
+    if (is_q || !PAGES) {
+        const RowsOut out = is_q ? a.q_out : is_v ? a.v_out : a.k_out;
+        uint8_t* dst = out.data;
+        int64_t head_stride = out.head_stride;
+        if (is_q && a.striped) {
+            const uint32_t ch = div((uint32_t)token0, a.pages.div_interleave), round = div(ch, a.pages.div_pcp);
+            const int64_t rank = ch - round * a.pages.pcp;
+            const int64_t local = (int64_t)round * a.pages.interleave + (token0 - (int64_t)ch * a.pages.interleave);
+            head_stride = (int64_t)a.local_q * D * 2;
+            dst += (rank * a.num_q_heads * a.local_q + local) * D * 2;
+        } else {
+            dst += token0 * out.token_stride;
+        }
+        dst += head0 * head_stride;
+        const int64_t step = dt ? out.token_stride : dh * head_stride, mine = r * head_stride + 2 * d0;
+#pragma unroll
+        for (int i = 0; i < NG; ++i, dst += step) {
+            if (!there(i) || !((live_mask >> (dt ? i : 0)) & 1)) continue;
+            *(v2i*)(dst + mine) = raw[i][0];
+            *(v2i*)(dst + mine + 2 * (d1 - d0)) = raw[i][1];
+        }
+        return;
+    }
+    if constexpr (PAGES) {
+        // ---- e4m3 codes of the k and v rows (of their bf16 values, rotated or not) -------------
+        float scale[NG];
+        uint32_t code[NG][2];
+        if constexpr (FP8) {
+            if (a.token_scales) {
+                // a row's largest finite magnitude, as a bf16 pattern (ordered as the
+                // integers are)
+                uint32_t m[NG], any = 0;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    m[i] = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t u = (uint32_t)raw[i][e >> 1][e & 1] & 0x7fff7fffu;
+                        m[i] = max(m[i], max(u >> 16, u & 0xffffu));
+                    }
+                    any = max(any, m[i]);
+                }
+                if (__builtin_amdgcn_ballot_w64(any >= 0x7f80u)) {
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        m[i] = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t u = ((uint32_t)raw[i][e >> 2][(e >> 1) & 1] >> (16 * (e & 1))) & 0x7fffu;
+                            m[i] = u < 0x7f80u ? max(m[i], u) : m[i];
+                        }
+                    }
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = x[e] / scale;
-                if (stored)
-                    *(v2i*)(a.pool + offset) = v2i{(int)cache::e4m3_codes4(x[0], x[1], x[2], x[3]),
-                                                   (int)cache::e4m3_codes4(x[4], x[5], x[6], x[7])};
-            } else if (stored) {
-                *(v4i*)(a.pool + offset) = raw;
+                for (int i = 0; i < NG; ++i) {
+                    m[i] = over_row<LANES>(m[i], [](uint32_t u, uint32_t v) { return max(u, v); });
+                    scale[i] = fmaxf(__uint_as_float(m[i] << 16) / kFp8Max, kScaleFloor);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) scale[i] = is_v ? a.v_scale : a.k_scale;
+            }
+            // as torch rounds x / scale (cache::div_rn: the same quotient in fewer
+            // instructions, where its range covers the scale)
+            const bool covered = a.token_scales || cache::div_rn_covers(is_v ? a.v_scale : a.k_scale);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                float x[8];
+                unpack(raw[i], x);
+                if (covered) {
+                    const float rcp = 1.f / scale[i];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = cache::div_rn(x[e], scale[i], rcp);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = x[e] / scale[i];
+                }
+                code[i][0] = cache::e4m3_codes4(x[0], x[1], x[2], x[3]);
+                code[i][1] = cache::e4m3_codes4(x[4], x[5], x[6], x[7]);
+            }
+        }
+        const int row0 = (is_v ? a.num_kv_heads : 0) + head0;  // of the page's K and V blocks
+        uint8_t* const heads_at = a.pool + row0 * a.pages.head_stride;
+        const int64_t mine = r * a.pages.head_stride + d0 * (FP8 ? 1 : 2);
+        float* const scales_at = a.token_scales + (int64_t)(row0 + r) * a.pages.block_size;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int page = __builtin_amdgcn_readlane(at.page, i), slot = __builtin_amdgcn_readlane(at.slot, i);
+            if (page < 0 || !there(i)) continue;
+            uint8_t* const dst = heads_at + page * a.pages.page_stride + (int64_t)slot * D * (FP8 ? 1 : 2) + mine;
+            if constexpr (FP8) {
+                *(uint32_t*)dst = code[i][0];
+                *(uint32_t*)(dst + (d1 - d0)) = code[i][1];
+                if (a.token_scales && c == 0)
+                    scales_at[(int64_t)page * 2 * a.num_kv_heads * a.pages.block_size + slot] = scale[i];
+            } else {
+                *(v2i*)dst = raw[i][0];
+                *(v2i*)(dst + 2 * (d1 - d0)) = raw[i][1];
             }
         }
     }
@@ -227,41 +396,71 @@ struct ReadArgs {
     float k_scale, v_scale;
 };
 
-// Thread: 8 values of one (token, head) row of K (grid z 0) or V (z 1).
+// A thread takes 8 values of kReads tokens' rows of one head of K (grid z 0) or V
+// (z 1): the table entries, then the rows and scales of all of them in flight.
+// The stores are whole lines and bypass the caches: what is read back is more
+// than they hold.  (131072 tokens, 2 heads at D 256 from e4m3 with token scales:
+// 76 us, 5.3 TB/s; with two stores of half lines each 129 us.)
+constexpr int kReads = 4;
+template <int D>
+constexpr int read_tokens() {  // tokens of a workgroup
+    return kTokenThreads / (D / 8) * kReads;
+}
 template <int D, bool FP8>
 __global__ void __launch_bounds__(kTokenThreads) cache_read_kernel(ReadArgs a) {
-    constexpr int LANES = D / 8;
-    const int64_t id = (int64_t)blockIdx.x * kTokenThreads + threadIdx.x;
-    const int token = (int)(id / LANES), c = (int)(id % LANES);
-    if (token >= a.num_tokens) return;
-    const int head = blockIdx.y, which = blockIdx.z;
-    const Place at = place_of(a.pages, 0, a.first_pos + token);
-    v4i out{0, 0, 0, 0};
-    if (at.page >= 0) {
-        const int hr = which * a.pages.num_kv_heads + head;
-        const uint8_t* const src = a.pool + at.page * a.pages.page_stride + (int64_t)hr * a.pages.head_stride;
-        if constexpr (FP8) {
-            const v2i raw = *(const v2i*)(src + (int64_t)at.slot * D + c * 8);
-            const float scale =
-                a.token_scales ? a.token_scales[((int64_t)at.page * 2 * a.pages.num_kv_heads + hr) *
-                                                    a.pages.block_size + at.slot]
-                               : which ? a.v_scale : a.k_scale;
-            float x[8];
+    constexpr int ROW = D * (FP8 ? 1 : 2), LANES = D / 8, AT_ONCE = kTokenThreads / LANES;
+    const int c = threadIdx.x % LANES;
+    const int64_t token0 = (int64_t)blockIdx.x * (AT_ONCE * kReads) + threadIdx.x / LANES;
+    const int head = blockIdx.y, which = blockIdx.z, hr = which * a.pages.num_kv_heads + head;
+    Place at[kReads];
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(raw[w], false);
-                const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(raw[w], true);
-                x[4 * w] = lo[0] * scale;
-                x[4 * w + 1] = lo[1] * scale;
-                x[4 * w + 2] = hi[0] * scale;
-                x[4 * w + 3] = hi[1] * scale;
-            }
-            out = to_bf16x8(x);
+    for (int u = 0; u < kReads; ++u) {
+        const int64_t token = token0 + u * AT_ONCE;
+        at[u] = token < a.num_tokens
+                    ? place_of(a.pages, 0, a.first_pos + token)
+                    : Place{-1, 0};
+    }
+    v4i raw[kReads];
+    float scale[kReads];
+#pragma unroll
+    for (int u = 0; u < kReads; ++u) {
+        raw[u] = v4i{0, 0, 0, 0};
+        scale[u] = which ? a.v_scale : a.k_scale;
+        if (at[u].page < 0) continue;
+        const uint8_t* const src = a.pool + at[u].page * a.pages.page_stride + (int64_t)hr * a.pages.head_stride +
+                                   (int64_t)at[u].slot * ROW + c * (ROW / LANES);
+        if constexpr (FP8) {
+            const v2i x = *(const v2i*)src;
+            raw[u][0] = x[0];
+            raw[u][1] = x[1];
+            if (a.token_scales)
+                scale[u] = a.token_scales[((int64_t)at[u].page * 2 * a.pages.num_kv_heads + hr) * a.pages.block_size +
+                                          at[u].slot];
         } else {
-            out = *(const v4i*)(src + ((int64_t)at.slot * D + c * 8) * 2);
+            raw[u] = *(const v4i*)src;
         }
     }
-    *(v4i*)((which ? a.v : a.k) + (((int64_t)head * a.num_tokens + token) * D + c * 8) * 2) = out;
+    uint8_t* const out = which ? a.v : a.k;
+#pragma unroll
+    for (int u = 0; u < kReads; ++u) {
+        const int64_t token = token0 + u * AT_ONCE;
+        if (token >= a.num_tokens) continue;
+        v4i x = raw[u];
+        if constexpr (FP8) {
+            float y[8];
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(raw[u][w], false);
+                const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(raw[u][w], true);
+                y[4 * w] = lo[0] * scale[u];
+                y[4 * w + 1] = lo[1] * scale[u];
+                y[4 * w + 2] = hi[0] * scale[u];
+                y[4 * w + 3] = hi[1] * scale[u];
+            }
+            x = to_bf16x8(y);
+        }
+        __builtin_nontemporal_store(x, (v4i*)(out + (((int64_t)head * a.num_tokens + token) * D + c * 8) * 2));
+    }
 }
 
 }  // namespace chunk
