@@ -80,7 +80,8 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
     };
     Span span, first_span;
     int length, tiles, walk, first_length, first_tiles, first_walk;
-    int64_t work = 0;
+    // (in 32-bit floats: only the range's length comes of them)
+    float work = 0.f, least = 0.f;
     for (int base = 0; base < a.chunk.batch; base += 64) {
         sequence(base, span, length, tiles, walk);
         if (base == 0) {
@@ -89,18 +90,19 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
             first_tiles = tiles;
             first_walk = walk;
         }
-        work += (int64_t)tiles * walk;
+        work += (float)tiles * (float)walk;
+        least += (float)tiles;
     }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) work += __shfl_xor(work, off);
-    const int64_t share = (work * heads + a.slots - 1) / a.slots;
-    int range = (int)max(share, (int64_t)a.min_range);
+    const float slots = (float)a.slots;
+    least = sum_over_lanes<64>(least) * heads;
+    const float share = ceilf(sum_over_lanes<64>(work) * heads / slots);
+    float length_of = fmaxf(fminf(share, 0x1p30f), (float)a.min_range);
     // Each sequence's last range is a shorter one, so that ranges of the fair
     // share are more than the GPU holds at once, and the few left over would run
-    // after all others: longer ranges, until all run together.  (64 sequences of
-    // 512 to 8192 tokens, 2 heads: NEWFIG.)
-    for (int tries = 0; tries < 6; ++tries) {
-        int64_t count = 0, least = 0;
+    // after all others: longer ranges, until all run together.  (64 sequences
+    // of 512 to 8192 tokens, 2 heads at D 256, e4m3: 83.2 -> 74.6 us.)
+    for (int tries = 0; tries < 6 && least < slots; ++tries) {
+        float count = 0.f;
         for (int base = 0; base < a.chunk.batch; base += 64) {
             if (base == 0) {
                 tiles = first_tiles;
@@ -108,17 +110,13 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
             } else {
                 sequence(base, span, length, tiles, walk);
             }
-            count += (int64_t)tiles * ((walk + range - 1) / range);
-            least += tiles;
+            count += (float)(tiles * ((walk + (int)length_of - 1) / (int)length_of));
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) {
-            count += __shfl_xor(count, off);
-            least += __shfl_xor(least, off);
-        }
-        if (count * heads <= a.slots || least * heads >= a.slots) break;
-        range = (int)min((int64_t)range + max((int64_t)1, range * (count * heads - a.slots) / a.slots), (int64_t)1 << 30);
+        count = sum_over_lanes<64>(count) * heads;
+        if (count <= slots) break;
+        length_of = fminf(ceilf(fmaxf(length_of + 1.f, length_of * (count / slots))), 0x1p30f);
     }
+    const int range = __builtin_amdgcn_readfirstlane((int)length_of);
     int before = 0;
     for (int base = 0; base < a.chunk.batch; base += 64) {
         if (base == 0) {
@@ -131,12 +129,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
         }
         const int ranges = (walk + range - 1) / range;
         const int items = tiles * heads * ranges;
-        int incl = items;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int up = __shfl_up(incl, off);
-            if (lane >= off) incl += up;
-        }
+        const int incl = inclusive_sum(items);
         const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > index);
         if (past) {
             const int src = __builtin_ctzll(past);
@@ -204,13 +197,13 @@ struct FewShape {
     static constexpr int V_BLOCKS = V_BYTES / 1024;  // DMA instructions of a step
     static constexpr int CH = ROW / 16;              // 16-byte chunks of a row
     // eight waves where their registers (256 each) and LDS hold it
-    static constexpr int WAVES = (D == 256 && (!FP8 || RT == 2)) || (D == 128 && !FP8) ? 4 : 8;
+    static constexpr int WAVES = D == 64 && !FP8 ? 8 : 4;
     static constexpr int THREADS = 64 * WAVES;
     static constexpr int O_ROW = D + 4;              // floats: 16 rows then start in all banks
     static constexpr int V_LDS = WAVES * 2 * V_BYTES;
     static constexpr int O_LDS = WAVES * 16 * O_ROW * 4;
     static constexpr int LDS = V_LDS > O_LDS ? V_LDS : O_LDS;
-    static constexpr int PER_CU = D == 64 && FP8 && RT == 1 ? 2 : 1;  // workgroups that fit
+    static constexpr int PER_CU = FP8 && !(D == 256 && RT == 2) ? 2 : 1;  // workgroups that fit
     static constexpr int ROWS = 16 * RT;
 };
 
@@ -234,6 +227,7 @@ struct FewStep {
     int page;     // -1: no step
     int slot;
     int u;
+    int entry;    // of the table
 };
 
 template <class S>
@@ -304,11 +298,12 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
     const const_i32_ptr table = (const_i32_ptr)(a.pages.table + (table_of(a.pages, it.b) << a.pages.table_shift));
     const int steps = (it.end - it.begin) * S::SUB;
-    // The wave's first step from step u on that has keys; page -1 past the last.
-    // (Steps without keys are passed over here, in scalar code: a loop body that
-    // may be skipped had two copies of O^T and K in registers.)
+    // The wave's first step from step u on that has keys, its page still a table
+    // entry to be read (entry -1: past the last).  Steps without keys are passed
+    // over here, in scalar code: a loop body that may be skipped had two copies
+    // of O^T and K in registers.
     auto step_from = [&](int u) {
-        FewStep<S> s{0, 0, 0, -1, 0, u};
+        FewStep<S> s{0, 0, 0, -1, 0, u, -1};
         for (; s.u < steps; s.u += S::WAVES) {
             const uint32_t tile = it.begin + s.u / S::SUB;
             const uint32_t lt = div(tile, a.pages.div_pcp);
@@ -317,14 +312,35 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
             const int n = min(owned(most_rounds, most_rest, rank) - local, S::KEYS);
             const uint32_t blk = div(local, a.pages.div_block);
             if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
-            const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
-            if ((unsigned)page >= (unsigned)a.pages.num_pages) continue;
             s.n = __builtin_amdgcn_readfirstlane(n);
             s.rank = __builtin_amdgcn_readfirstlane(rank);
             s.local = __builtin_amdgcn_readfirstlane(local);
-            s.page = __builtin_amdgcn_readfirstlane(page);
+            s.entry = __builtin_amdgcn_readfirstlane(rank * a.pages.max_local_blocks + (int)blk);
             s.slot = __builtin_amdgcn_readfirstlane(local - (int)blk * a.pages.block_size);
             break;
+        }
+        return s;
+    };
+    // Its table entry, read ahead (the two dwords of an int64 one).
+    struct Entry {
+        int lo, hi;
+    };
+    auto read_entry = [&](const FewStep<S>& s) {
+        const int i = max(s.entry, 0) << a.pages.table_shift;
+        return Entry{table[i], table[i + a.pages.table_shift]};
+    };
+    auto page_of = [&](const Entry& e) {
+        const bool good = (unsigned)e.lo < (unsigned)a.pages.num_pages && !(a.pages.table_shift && e.hi != 0);
+        return good ? e.lo : -1;
+    };
+    // The step with its page, from what was read ahead; steps without a page are
+    // passed over.
+    auto with_page = [&](FewStep<S> s, Entry e) {
+        while (s.entry >= 0) {
+            s.page = page_of(e);
+            if (s.page >= 0) break;
+            s = step_from(s.u + S::WAVES);
+            e = read_entry(s);
         }
         return s;
     };
@@ -398,8 +414,14 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
         for (int dt = 0; dt < DT; ++dt) o[rt][dt] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    // ---- the walk: the step after next is looked up, the next loads, this one runs ----
-    FewStep<S> st = step_from(wave), nxt = step_from(st.u + S::WAVES);
+    // ---- the walk: two steps on a table entry is read, the next step's keys load, this one
+    // runs ----
+    FewStep<S> ahead = step_from(wave);
+    FewStep<S> st = with_page(ahead, read_entry(ahead));
+    ahead = step_from(st.u + S::WAVES);
+    FewStep<S> nxt = with_page(ahead, read_entry(ahead));
+    ahead = step_from(nxt.u + S::WAVES);
+    Entry entry = read_entry(ahead);
     issue_v(st, my_addr);
     issue_k(st);
     issue_scales(st);
@@ -408,7 +430,9 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
         wait_vmem();
         __builtin_amdgcn_sched_barrier(0);
         issue_v(nxt, my_addr + (buf ^ S::V_BYTES));
-        const FewStep<S> after = step_from(nxt.u + S::WAVES);
+        const FewStep<S> after = with_page(ahead, entry);
+        ahead = step_from(after.u + S::WAVES);
+        entry = read_entry(ahead);
         // ---- scores -----------------------------------------------------------
         v4f s[RT][2 * KG];
 #pragma unroll
@@ -684,30 +708,27 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
 
     // ---- this lane's row and what it sees ------------------------------------------
     const int rows = it.span.count * a.group, row0 = it.tile * kRowsPerGroup;
-    const int row = row0 + pw * kRowsPerWave + j;
-    const bool row_ok = row < rows;
-    const int row_c = min(row, rows - 1);  // rows past the last do as the last, unseen
+    // (rows past the last do as the last, unseen)
+    const int row_c = min(row0 + pw * kRowsPerWave + j, rows - 1);
     const int64_t len = a.chunk.lengths[it.b];
     auto sees = [&](int r) {
         const int64_t np = len - it.span.count + r / a.group + 1;
         return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
     };
-    const int64_t row_index = (int64_t)(it.span.first + row_c / a.group) * a.num_q_heads + it.head * a.group + row_c % a.group;
-    const int stride = a.pages.pcp * a.pages.interleave;
+    auto index_of = [&](int r) {
+        return (int64_t)(it.span.first + r / a.group) * a.num_q_heads + it.head * a.group + r % a.group;
+    };
     const int seen = sees(row_c);
-    const int rounds = seen / stride * a.pages.interleave, rest = seen % stride;
     const int most = __builtin_amdgcn_readfirstlane(sees(min(row0 + kRowsPerGroup, rows) - 1));
     const int least = __builtin_amdgcn_readfirstlane(sees(row0));
-    const int most_rounds = most / stride * a.pages.interleave, most_rest = most % stride;
-    const int least_rounds = least / stride * a.pages.interleave, least_rest = least % stride;
-    auto owned = [&](int whole, int tail, int rank) {
-        return whole + min(max(tail - rank * a.pages.interleave, 0), a.pages.interleave);
-    };
     v8bf qop[QK];
+    {
+        const uint8_t* const qrow = a.q + index_of(row_c) * D * 2;
 #pragma unroll
-    for (int c = 0; c < QK; ++c) {
-        const int d = S::WIDE ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h;
-        qop[c] = __builtin_bit_cast(v8bf, *(const v4i*)(a.q + (row_index * D + d) * 2));
+        for (int c = 0; c < QK; ++c) {
+            const int d = S::WIDE ? 32 * (c >> 1) + 16 * h + 8 * (c & 1) : 16 * c + 8 * h;
+            qop[c] = __builtin_bit_cast(v8bf, *(const v4i*)(qrow + d * 2));
+        }
     }
 
     // ---- per-lane LDS and DMA offsets (the tile kernel's maps) ------------------------
@@ -728,11 +749,6 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
                            (dbyte & 15) + kh * 32 * ROW;
         }
     }
-    {
-        const int byte = wave * 1024 + lane * 16, r = byte / ROW, pos = (byte % ROW) / 16;
-        L.dma_off = lds_row<F8>(r) * ROW + (pos ^ chunk_swizzle<F8, CHUNKS>(r)) * 16;
-        L.dma_off_v = lds_row<F8>(r) * ROW + (pos ^ chunk_swizzle_v<F8, CHUNKS>(r)) * 16;
-    }
 
     // ---- the walk ------------------------------------------------------------------------
     typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
@@ -743,7 +759,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         for (; t.i < end; ++t.i) {
             const uint32_t lt = div((uint32_t)t.i, a.pages.div_pcp);
             const int rank = t.i - lt * a.pages.pcp, local = lt * kKeyTile;
-            const int n = min(owned(most_rounds, most_rest, rank) - local, kKeyTile);
+            const int n = min(owned_of(a.pages, most, rank) - local, kKeyTile);
             const uint32_t blk = div((uint32_t)local, a.pages.div_block);
             if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
             const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
@@ -763,7 +779,16 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     f.num_kv_heads = a.pages.num_kv_heads;
     // the thread's scale of tile t: threads 0 .. 63 K's, 64 .. 127 V's (TWO: the
     // next 128 the second tile's); slots without a token hold none
+    // (opaque here and below: what a thread's index gives is formed where it is used;
+    // kept over the walk it cost Q's registers, parts of which were then read back
+    // from memory for every tile)
+    auto thread = [&]() {
+        int x = tid;
+        asm volatile("" : "+v"(x));
+        return x;
+    };
     auto load_scale = [&](const ManyTile& t, const ManyTile& t2) {
+        const int tid = thread();
         const bool other = TWO && (tid & 128);
         const int page = other ? t2.page : t.page, slot = other ? t2.slot : t.slot, n = other ? t2.n : t.n;
         const int key = tid & 63, which = (tid >> 6) & 1;
@@ -784,38 +809,37 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     // see their keys after the walk.  Called by the whole workgroup.
     bool spoiled = false;
     auto settle_v = [&](uint8_t* v, const ManyTile& t) {
-        const int from = max(owned(least_rounds, least_rest, t.rank) - t.local, 0);
-        if (t.n < kKeyTile) zero_masked_v<S>(v, t.n, tid);
+        const int tid = thread();
+        const int from = max(owned_of(a.pages, least, t.rank) - t.local, 0);
         bool bad = false;
-        for (int i = from * CHUNKS + tid; i < t.n * CHUNKS; i += S::THREADS) {
+        for (int i = from * CHUNKS + tid; i < kKeyTile * CHUNKS; i += S::THREADS) {
             v4i* const at = (v4i*)(v + lds_row<F8>(i / CHUNKS) * ROW + (i % CHUNKS) * 16);
-            v4i x = *at;
-            bool here = false;
+            const v4i x = *at;
+            const uint32_t keep = i < t.n * CHUNKS ? ~0u : 0u;
+            v4i y;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t u = (uint32_t)x[w];
-                if constexpr (F8) {
-#pragma unroll
-                    for (int b = 0; b < 32; b += 8)
-                        if (((u >> b) & 0x7fu) == 0x7fu) u &= ~(0xffu << b);
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 32; b += 16)
-                        if (((u >> b) & 0x7f80u) == 0x7f80u) u &= ~(0xffffu << b);
-                }
-                here |= u != (uint32_t)x[w];
-                x[w] = (int)u;
+                // the values whose exponent (code) is all ones: a carry into their sign bit
+                const uint32_t u = (uint32_t)x[w];
+                const uint32_t ones = F8 ? (((u & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7
+                                         : (((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15;
+                y[w] = (int)(u & ~(ones * (F8 ? 0xffu : 0xffffu)) & keep);
+                bad |= ones != 0 && keep != 0;
             }
-            if (here) *at = x;
-            bad |= here;
+            *at = y;
         }
         spoiled |= __syncthreads_or(bad) != 0;
     };
-    auto settled = [&](const ManyTile& t) { return owned(least_rounds, least_rest, t.rank) - t.local >= kKeyTile; };
+    auto settled = [&](const ManyTile& t) { return owned_of(a.pages, least, t.rank) - t.local >= kKeyTile; };
 
     ManyTile cur = tile_from(it.begin), cur2{}, nxt, nxt2{};
     float scale = 0.f;
     auto stage = [&](const ManyTile& t, const ManyTile& t2, uint8_t* buf) {
+        {
+            const int byte = wave * 1024 + (thread() & 63) * 16, r = byte / ROW, pos = (byte % ROW) / 16;
+            L.dma_off = lds_row<F8>(r) * ROW + (pos ^ chunk_swizzle<F8, CHUNKS>(r)) * 16;
+            L.dma_off_v = lds_row<F8>(r) * ROW + (pos ^ chunk_swizzle_v<F8, CHUNKS>(r)) * 16;
+        }
         if (t.page >= 0) stage_tile_async<S>(f, TileCursor{0, t.slot, 0, t.page * a.pages.page_stride}, buf, wave, L);
         if (TWO && t2.page >= 0)
             stage_tile_async<S>(f, TileCursor{0, t2.slot, 0, t2.page * a.pages.page_stride}, buf + 2 * S::TILE, wave, L);
@@ -829,24 +853,28 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         const uint32_t rt_off = rbuf * S::BUFFER;
         wait_vmem();  // this wave's loads of the current tiles have landed
         float* const sc = scales + rbuf * S::TILES * 2 * kKeyTile;
-        if (SCALED && tid < 128 * S::TILES) sc[tid] = scale;
+        if (const int t = thread(); SCALED && t < 128 * S::TILES) sc[t] = scale;
         __syncthreads();  // ... and every wave's; the other buffer is free
         stage(nxt, nxt2, lds + (rt_off ^ S::BUFFER));
         if (!settled(cur)) settle_v(lds + rt_off + S::TILE, cur);
         if (TWO && cur2.page >= 0 && !settled(cur2)) settle_v(lds + rt_off + 3 * S::TILE, cur2);
+        const int hl = (thread() >> 5) & 1;
         if constexpr (TWO) {
             const ManyTile& t = kh ? cur2 : cur;
             if (t.page >= 0)
-                compute_tile<S, 0, true, SCALED>(lds, rt_off + kh * 2 * S::TILE, owned(rounds, rest, t.rank) - t.local,
-                                                 qop, a.score_scale, L, h, st, sc + kh * 2 * kKeyTile);
+                compute_tile<S, 0, true, SCALED>(lds, rt_off + kh * 2 * S::TILE, owned_of(a.pages, seen, t.rank) - t.local,
+                                                 qop, a.score_scale, L, hl, st, sc + kh * 2 * kKeyTile);
         } else {
             const int first_key = S::PAIR ? 32 * kh : 0;
-            compute_tile<S, 0, true, SCALED>(lds, rt_off, owned(rounds, rest, cur.rank) - cur.local - first_key, qop,
-                                             a.score_scale, L, h, st, sc);
+            compute_tile<S, 0, true, SCALED>(lds, rt_off, owned_of(a.pages, seen, cur.rank) - cur.local - first_key, qop,
+                                             a.score_scale, L, hl, st, sc);
         }
         cur = nxt;
         cur2 = nxt2;
     }
+
+    const int lane2 = thread() & 63, h2 = lane2 >> 5;
+    const int row = row0 + pw * kRowsPerWave + (lane2 & 31);
 
     // ---- PAIR: the two waves' results meet in the first wave of the pair ----------------
     if constexpr (S::PAIR) {
@@ -857,21 +885,21 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
             for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4)
-                    *(v4f*)(xo + ((4 * dt + r4) * 64 + lane) * 4) =
+                    *(v4f*)(xo + ((4 * dt + r4) * 64 + lane2) * 4) =
                         v4f{st.o[dt][4 * r4], st.o[dt][4 * r4 + 1], st.o[dt][4 * r4 + 2], st.o[dt][4 * r4 + 3]};
-            pair_ml[(pw * 64 + lane) * 2] = st.m;
-            pair_ml[(pw * 64 + lane) * 2 + 1] = st.l;
+            pair_ml[(pw * 64 + lane2) * 2] = st.m;
+            pair_ml[(pw * 64 + lane2) * 2 + 1] = st.l;
         }
         __syncthreads();
         if (kh == 1) return;
-        const float m1 = pair_ml[(pw * 64 + lane) * 2], l1 = pair_ml[(pw * 64 + lane) * 2 + 1];
+        const float m1 = pair_ml[(pw * 64 + lane2) * 2], l1 = pair_ml[(pw * 64 + lane2) * 2 + 1];
         const float m = fmaxf(st.m, m1);
         const float w0 = __builtin_amdgcn_exp2f(st.m - m), w1 = __builtin_amdgcn_exp2f(m1 - m);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4) {
-                const v4f x = *(const v4f*)(xo + ((4 * dt + r4) * 64 + lane) * 4);
+                const v4f x = *(const v4f*)(xo + ((4 * dt + r4) * 64 + lane2) * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) st.o[dt][4 * r4 + i] = fmaf(w1, x[i], w0 * st.o[dt][4 * r4 + i]);
             }
@@ -882,10 +910,10 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     // ---- values that are not finite, for the rows that see them (from the pages) -----------
     if (spoiled) {
         for (ManyTile t = tile_from(it.begin); t.page >= 0; t = tile_from(t.i + 1)) {
-            const int vis = min(owned(rounds, rest, t.rank) - t.local, t.n);
-            for (int key = max(owned(least_rounds, least_rest, t.rank) - t.local, 0); key < t.n; ++key) {
+            const int vis = min(owned_of(a.pages, sees(min(row, rows - 1)), t.rank) - t.local, t.n);
+            for (int key = max(owned_of(a.pages, least, t.rank) - t.local, 0); key < t.n; ++key) {
                 const uint8_t* const v = f.kv + t.page * a.pages.page_stride + a.pages.num_kv_heads * a.pages.head_stride +
-                                         (int64_t)(t.slot + key) * ROW + 4 * h * S::ES;
+                                         (int64_t)(t.slot + key) * ROW + 4 * h2 * S::ES;
                 if (key >= vis) continue;
                 static_for<0, 4 * DT>([&](auto c) {
                     constexpr int dt = decltype(c)::value >> 2, r4 = decltype(c)::value & 3;
@@ -899,6 +927,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
                             x = bf16_bits_to_f32(((const uint16_t*)v)[d]);
                         if (!(fabsf(x) < INFINITY)) st.o[dt][4 * r4 + i] += x;
                     }
+                    __builtin_amdgcn_sched_barrier(0);  // (few registers for this rare path)
                 });
             }
         }
@@ -909,16 +938,17 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     const bool empty = total == 0.f;
     const float inv = empty ? 0.f : a.v_scale / total;
     const float log2sum = empty ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
-    if (!row_ok) return;
+    if (row >= rows) return;
+    const int64_t row_index = index_of(row);
     const bool part = it.plan.ranges > 1;
-    const int64_t prow = (int64_t)blockIdx.x * kRowsPerGroup + pw * kRowsPerWave + j;
+    const int64_t prow = (int64_t)blockIdx.x * kRowsPerGroup + pw * kRowsPerWave + (lane2 & 31);
     float* const po = a.part_o + prow * D;
     uint8_t* const orow = a.out + row_index * D * 2;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-            const int d = 32 * dt + 8 * r4 + 4 * h;
+            const int d = 32 * dt + 8 * r4 + 4 * h2;
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = empty ? 0.f : st.o[dt][4 * r4 + i] * inv;
@@ -935,7 +965,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
                 *(v2i*)(orow + 2 * d) = v2i{(int)w[0], (int)w[1]};
             }
         }
-    if (h == 0) {
+    if (h2 == 0) {
         if (part)
             a.part_lse[prow] = log2sum;
         else if (a.lse)
@@ -1026,18 +1056,21 @@ __global__ void __launch_bounds__(256) merge_few_ranges_kernel(AttendArgs a) {
     }
 }
 
-// Rows with many ranges: a workgroup of 16 waves per (row, Q head), 1024 / (D / 4)
-// partials at a time, which meet in LDS.
+// Rows with many ranges: a workgroup of 16 waves per 64 values of a (row, Q
+// head), 64 partials at a time, 16 lanes to each; the four of a wave meet in
+// registers, the waves in LDS.  (32 rows of 256 ranges at D 256: MERGEFIG.)
+constexpr int kMergeParts = 64;  // values of a workgroup
 template <int D>
 __global__ void __launch_bounds__(1024) merge_many_ranges_kernel(AttendArgs a) {
-    constexpr int LANES = D / 4, AT_ONCE = 1024 / LANES, UNROLL = 4;
-    __shared__ v4f part[AT_ONCE][LANES];
-    __shared__ float part_ml[AT_ONCE][2];
+    constexpr int LANES = kMergeParts / 4, AT_ONCE = 1024 / LANES, UNROLL = 4, WAVES = 16;
+    __shared__ v4f part[WAVES][LANES];
+    __shared__ float part_ml[WAVES][2];
     const int token = blockIdx.x, head = blockIdx.y;
     const int b = sequence_of(a.chunk, token);
     Partials p;
     if (!partials_of(a, b, token, head, p)) return;
-    const int at = threadIdx.x / LANES, c = threadIdx.x % LANES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x / LANES, c = threadIdx.x % LANES;
+    const int value = blockIdx.z * kMergeParts + 4 * c;
     Merged r{-INFINITY, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
     for (int s0 = at; s0 < p.ranges; s0 += AT_ONCE * UNROLL) {
         float ls[UNROLL];
@@ -1046,32 +1079,39 @@ __global__ void __launch_bounds__(1024) merge_many_ranges_kernel(AttendArgs a) {
         for (int u = 0; u < UNROLL; ++u) {
             const int64_t row = p.first + min(s0 + u * AT_ONCE, p.ranges - 1) * p.step;
             ls[u] = a.part_lse[row];
-            x[u] = *(const v4f*)(a.part_o + row * D + 4 * c);
+            x[u] = *(const v4f*)(a.part_o + row * D + value);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) r.add(s0 + u * AT_ONCE < p.ranges ? ls[u] : -INFINITY, x[u]);
     }
-    part[at][c] = r.acc;
-    if (c == 0) {
-        part_ml[at][0] = r.top;
-        part_ml[at][1] = r.total;
+    // (a partial that saw nothing weighs nothing; one that is NaN has a NaN total)
+    float top = quarters_max(r.top);
+    float weight = r.total == 0.f ? 0.f : __builtin_amdgcn_exp2f(r.top - top);
+    float total = quarters_sum(weight * r.total);
+    v4f acc;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] = quarters_sum(weight * r.acc[k]);
+    if (lane < LANES) part[wave][c] = acc;
+    if (lane == 0) {
+        part_ml[wave][0] = top;
+        part_ml[wave][1] = total;
     }
     __syncthreads();
-    if (at != 0) return;
-    const int n = min(p.ranges, AT_ONCE);
-    float top = part_ml[0][0];
-    for (int i = 1; i < n; ++i) top = fmaxf(top, part_ml[i][0]);
-    float total = 0.f;
-    v4f acc{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < n; ++i) {
-        if (part_ml[i][1] == 0.f) continue;  // nothing seen (a NaN is not nothing)
-        const float weight = __builtin_amdgcn_exp2f(part_ml[i][0] - top);
+    if (threadIdx.x >= LANES) return;
+    top = part_ml[0][0];
+#pragma unroll
+    for (int i = 1; i < WAVES; ++i) top = fmaxf(top, part_ml[i][0]);
+    total = 0.f;
+    acc = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+        weight = part_ml[i][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(part_ml[i][0] - top);
         total = fmaf(weight, part_ml[i][1], total);
         const v4f x = part[i][c];
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] = fmaf(weight, x[k], acc[k]);
     }
-    store_merged<D>(a, (int64_t)token * a.num_q_heads + head, c, top, total, acc);
+    store_merged<D>(a, (int64_t)token * a.num_q_heads + head, value / 4, top, total, acc);
 }
 
 }  // namespace chunk

@@ -60,6 +60,49 @@ inline Div make_div(uint32_t d) {
 }
 __device__ __forceinline__ uint32_t div(uint32_t n, const Div& d) { return (uint32_t)(((uint64_t)n * d.m) >> d.shift); }
 
+// Over the 64 lanes, by DPP within 16 lanes and by row and half swaps beyond
+// (the shuffles go through LDS, ten times the wait).  f has to be commutative;
+// every lane gets the result, formed in the same order in every wave.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);
+}
+// ... over LANES (8, 16, 32 or 64) neighbouring lanes.
+template <int LANES, class F>
+__device__ __forceinline__ uint32_t over_lanes(uint32_t x, F f) {
+    x = f(x, dpp<0xB1>(x));   // lane ^ 1
+    x = f(x, dpp<0x4E>(x));   // lane ^ 2
+    x = f(x, dpp<0x141>(x));  // half rows mirrored: lane 7 - i of 8
+    if constexpr (LANES >= 16) x = f(x, dpp<0x140>(x));  // rows mirrored: lane 15 - i of 16
+    if constexpr (LANES >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        x = f(r[0], r[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        x = f(r[0], r[1]);
+    }
+    return x;
+}
+template <int LANES>
+__device__ __forceinline__ float sum_over_lanes(float x) {
+    return __uint_as_float(over_lanes<LANES>(__float_as_uint(x), [](uint32_t u, uint32_t v) {
+        return __float_as_uint(__uint_as_float(u) + __uint_as_float(v));
+    }));
+}
+// Inclusive sums over the lanes before and at each lane.
+__device__ __forceinline__ int inclusive_sum(int x) {
+    const int lane = threadIdx.x & 63;
+    // row_shr:1, 2, 4, 8 (lanes without a source add 0)
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    const int r0 = __builtin_amdgcn_readlane(x, 15), r1 = __builtin_amdgcn_readlane(x, 31);
+    const int r2 = __builtin_amdgcn_readlane(x, 47);
+    return x + (lane >= 48 ? r0 + r1 + r2 : lane >= 32 ? r0 + r1 : lane >= 16 ? r0 : 0);
+}
+
 struct Pages {
     const int32_t* table;  // [batch, pcp, max_local_blocks], int32 or int64 as dword pairs
     int32_t table_shift;
@@ -69,7 +112,7 @@ struct Pages {
     int32_t pcp;
     int32_t interleave;
     int32_t num_kv_heads;
-    Div div_interleave, div_pcp, div_block;
+    Div div_interleave, div_pcp, div_block, div_stride;  // (stride: pcp * interleave)
     int32_t capacity;      // positions of a sequence's cache: pcp * max_local_blocks * block_size
     int64_t page_stride;   // bytes of a page
     int64_t head_stride;   // bytes of one head's K (or V) of a page
@@ -84,6 +127,13 @@ __device__ __forceinline__ int page_at(const Pages& p, int64_t first, int e) {
     return good ? page : -1;
 }
 __device__ __forceinline__ int64_t table_of(const Pages& p, int b) { return (int64_t)b * p.pcp * p.max_local_blocks; }
+
+// Positions [0, keys) that rank `rank` holds: paging::owned_below for 0 <= keys < 2^31.
+__device__ __forceinline__ int owned_of(const Pages& p, int keys, int rank) {
+    const int round = (int)div((uint32_t)keys, p.div_stride);
+    const int rest = keys - round * (p.pcp * p.interleave);
+    return round * p.interleave + min(max(rest - rank * p.interleave, 0), p.interleave);
+}
 
 // Page and slot of position `pos` (page -1: none) in the table at `first`.
 struct Place {

@@ -213,7 +213,7 @@ __device__ __forceinline__ float halves_sum(float x) {
 //   BF16 (one PV MFMA eats 16 keys, 8 per lane half):
 //        key = 32t + 16*(r/8) + 8h + r%8
 template <bool FP8>
-__device__ __forceinline__ int key_of_acc(int t, int r, int h) {
+__device__ __forceinline__ constexpr int key_of_acc(int t, int r, int h) {
     return FP8 ? 32 * h + 16 * t + r : 32 * t + 16 * (r >> 3) + 8 * h + (r & 7);
 }
 // Same map indexed by the A-operand row rho (0..31) of the score MFMA.
@@ -368,6 +368,13 @@ __device__ __forceinline__ v2i ds_read_tr16_b64(uint32_t addr) {
     return r;
 }
 template <int OFF>
+__device__ __forceinline__ v2i ds_read_b64(uint32_t addr) {
+    static_assert(OFF >= 0 && OFF < 65536, "ds offset is 16 bits");
+    v2i r;
+    asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "i"(OFF));
+    return r;
+}
+template <int OFF>
 __device__ __forceinline__ v4i ds_read_b128(uint32_t addr) {
     static_assert(OFF >= 0 && OFF < 65536, "ds offset is 16 bits");
     v4i r;
@@ -378,6 +385,10 @@ __device__ __forceinline__ v4i ds_read_b128(uint32_t addr) {
 // no use of them is scheduled before the wait.
 template <int N>
 __device__ __forceinline__ void lds_wait(v4i& x) {
+    asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(x) : "i"(N));
+}
+template <int N>
+__device__ __forceinline__ void lds_wait(v2i& x) {
     asm volatile("s_waitcnt lgkmcnt(%1)" : "+v"(x) : "i"(N));
 }
 template <int N>

@@ -56,6 +56,7 @@ Pages pages_of(const pcpa_params* p, int32_t interleave, const void* block_table
     g.div_interleave = make_div((uint32_t)interleave);
     g.div_pcp = make_div((uint32_t)p->pcp_size);
     g.div_block = make_div((uint32_t)p->block_size);
+    g.div_stride = make_div((uint32_t)p->pcp_size * (uint32_t)interleave);
     g.capacity = (int32_t)((int64_t)p->pcp_size * p->max_local_blocks * p->block_size);
     g.head_stride = (int64_t)p->block_size * p->head_dim * es;
     g.page_stride = 2 * (int64_t)p->num_kv_heads * g.head_stride;
@@ -286,7 +287,8 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
                               : p->head_dim == 128 ? merge_kernel_for<128>(many)
                                                    : merge_kernel_for<256>(many);
     const int at_once = 256 / (p->head_dim / 4);
-    const dim3 grid(c->num_tokens, many ? p->num_q_heads : (p->num_q_heads + at_once - 1) / at_once);
+    const dim3 grid(c->num_tokens, many ? p->num_q_heads : (p->num_q_heads + at_once - 1) / at_once,
+                    many ? p->head_dim / kMergeParts : 1);
     return hipLaunchKernel(merge, grid, dim3(many ? 1024 : 256), args, 0, stream) == hipSuccess ? PCPA_OK
                                                                                                : PCPA_ERR_LAUNCH;
 }

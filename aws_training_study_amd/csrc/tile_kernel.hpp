@@ -126,6 +126,28 @@ struct SoftmaxState {
 template <class S>
 using QOperand = typename std::conditional<S::MFMA8, v8i, v8bf>::type;
 
+// The scores (or probabilities) of two score tiles times their keys' factors
+// from LDS, read two at a time, one read ahead (beside O^T, Q and the scores there
+// is no room for more: with four, parts of Q went to memory).
+template <bool FP8>
+__device__ __forceinline__ void scale_scores(v16f (&s)[2], const float* factors, int h) {
+    const uint32_t base = lds_address((const uint8_t*)factors) + 4 * key_of_acc<FP8>(0, 0, h);
+    v2i x[2];
+    auto read = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        x[i & 1] = ds_read_b64<4 * (key_of_acc<FP8>(i >> 3, 2 * (i & 7), 0))>(base);
+    };
+    read(std::integral_constant<int, 0>{});
+    static_for<0, 16>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if constexpr (i + 1 < 16) read(std::integral_constant<int, i + 1>{});
+        lds_wait<(i + 1 < 16 ? 1 : 0)>(x[i & 1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s[i >> 3][2 * (i & 7) + e] *= __int_as_float(x[i & 1][e]);
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
+
 // One 64-key tile held in LDS buffer BUF (PAIR_HALVES: this wave's 32 keys of
 // it; its operand addresses in L include the half): S^T = K Q^T, masked online
 // softmax, O^T += V^T P^T.  `valid`: the valid keys counted from the wave's
@@ -224,14 +246,7 @@ __device__ __forceinline__ void compute_tile(const uint8_t* lds, uint32_t rt_off
     __builtin_amdgcn_s_setprio(S::PAIR ? 0 : 1);
     if constexpr (SCALED) {
         static_assert(S::WIDE, "scales go with e4m3 tiles and bf16 MFMAs");
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const v4f x = *(const v4f*)(scales + key_of_acc<F8>(t, 4 * r4, h));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[t][4 * r4 + i] *= x[i];
-            }
+        scale_scores<F8>(s, scales, h);
     }
     // ---- mask, online softmax (lazy rescale) ----------------------------
     // (CAUSAL: only tiles that cross some row's limit, a wave-uniform test)
@@ -274,16 +289,7 @@ __device__ __forceinline__ void compute_tile(const uint8_t* lds, uint32_t rt_off
             s[t][r] = p;
             if constexpr (!FP8) psum += p;
         }
-    if constexpr (SCALED) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const v4f x = *(const v4f*)(scales + kKeyTile + key_of_acc<F8>(t, 4 * r4, h));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[t][4 * r4 + i] *= x[i];
-            }
-    }
+    if constexpr (SCALED) scale_scores<F8>(s, scales + kKeyTile, h);
     // BF16: this lane half's share of the row sum, from the unrounded P (the
     // bf16 rounding of P below is 2^-9 relative).  FP8: the full row sum of
     // the e4m3-rounded P that the PV MFMAs consume, taken by an MFMA below.

@@ -61,32 +61,6 @@ __device__ __forceinline__ v4i to_bf16x8(const float (&x)[8]) {
     }
     return r;
 }
-// Sum / maximum over the LANES (8, 16 or 32) neighbouring lanes of a row:
-// exchanges within 16 lanes by DPP (quads, halves and rows mirrored once the
-// smaller groups agree), then lanes 16 apart by a row swap.
-template <int CTRL>
-__device__ __forceinline__ uint32_t dpp(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, true);
-}
-template <int LANES, class F>
-__device__ __forceinline__ uint32_t over_row(uint32_t x, F f) {
-    x = f(x, dpp<0xB1>(x));   // lane ^ 1
-    x = f(x, dpp<0x4E>(x));   // lane ^ 2
-    x = f(x, dpp<0x141>(x));  // half rows mirrored: lane 7 - i of 8
-    if constexpr (LANES >= 16) x = f(x, dpp<0x140>(x));  // rows mirrored: lane 15 - i of 16
-    if constexpr (LANES >= 32) {
-        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        x = f(r[0], r[1]);
-    }
-    return x;
-}
-template <int LANES>
-__device__ __forceinline__ float sum_over_row(float x) {
-    return __uint_as_float(over_row<LANES>(__float_as_uint(x), [](uint32_t u, uint32_t v) {
-        return __float_as_uint(__uint_as_float(u) + __uint_as_float(v));
-    }));
-}
-
 __host__ __device__ constexpr int token_rows(int d) { return 64 / (d / 8); }  // rows of a group
 
 // A group is 64 / (D / 8) heads of one token's Q, K or V, a row's D values 8 to
@@ -252,7 +226,7 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(TokenArgs a) {
                 float sum = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
-                sum = sum_over_row<LANES>(sum);
+                sum = sum_over_lanes<LANES>(sum);
                 const float inv = __builtin_amdgcn_rsqf(sum * (1.f / D) + a.norm_eps);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] *= inv * w8[e];
@@ -337,7 +311,7 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(TokenArgs a) {
                 }
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
-                    m[i] = over_row<LANES>(m[i], [](uint32_t u, uint32_t v) { return max(u, v); });
+                    m[i] = over_lanes<LANES>(m[i], [](uint32_t u, uint32_t v) { return max(u, v); });
                     scale[i] = fmaxf(__uint_as_float(m[i] << 16) / kFp8Max, kScaleFloor);
                 }
             } else {
