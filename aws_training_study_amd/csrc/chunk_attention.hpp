@@ -166,6 +166,21 @@ __device__ __forceinline__ float quarters_sum(float x) {
     return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// A table entry as it is read ahead (the two dwords of an int64 one; entry 0 in
+// the place of none), and its page, or -1.
+typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
+struct TableEntry {
+    int lo, hi;
+};
+__device__ __forceinline__ TableEntry entry_of(const_i32_ptr table, const Pages& p, int entry) {
+    const int64_t i = (int64_t)max(entry, 0) << p.table_shift;
+    return TableEntry{table[i], table[i + p.table_shift]};
+}
+__device__ __forceinline__ int page_of(const Pages& p, const TableEntry& e) {
+    const bool good = (unsigned)e.lo < (unsigned)p.num_pages && !(p.table_shift && e.hi != 0);
+    return good ? e.lo : -1;
+}
+
 // ---- few rows ------------------------------------------------------------------
 //
 // For up to 32 rows per (sequence, KV head) - one token of a GQA group, or a few
@@ -295,7 +310,6 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     };
 
     // ---- the wave's steps ----------------------------------------------------------
-    typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
     const const_i32_ptr table = (const_i32_ptr)(a.pages.table + (table_of(a.pages, it.b) << a.pages.table_shift));
     const int steps = (it.end - it.begin) * S::SUB;
     // The wave's first step from step u on that has keys, its page still a table
@@ -321,23 +335,12 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
         }
         return s;
     };
-    // Its table entry, read ahead (the two dwords of an int64 one).
-    struct Entry {
-        int lo, hi;
-    };
-    auto read_entry = [&](const FewStep<S>& s) {
-        const int i = max(s.entry, 0) << a.pages.table_shift;
-        return Entry{table[i], table[i + a.pages.table_shift]};
-    };
-    auto page_of = [&](const Entry& e) {
-        const bool good = (unsigned)e.lo < (unsigned)a.pages.num_pages && !(a.pages.table_shift && e.hi != 0);
-        return good ? e.lo : -1;
-    };
+    auto read_entry = [&](const FewStep<S>& s) { return entry_of(table, a.pages, s.entry); };
     // The step with its page, from what was read ahead; steps without a page are
     // passed over.
-    auto with_page = [&](FewStep<S> s, Entry e) {
+    auto with_page = [&](FewStep<S> s, TableEntry e) {
         while (s.entry >= 0) {
-            s.page = page_of(e);
+            s.page = page_of(a.pages, e);
             if (s.page >= 0) break;
             s = step_from(s.u + S::WAVES);
             e = read_entry(s);
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     ahead = step_from(st.u + S::WAVES);
     FewStep<S> nxt = with_page(ahead, read_entry(ahead));
     ahead = step_from(nxt.u + S::WAVES);
-    Entry entry = read_entry(ahead);
+    TableEntry entry = read_entry(ahead);
     issue_v(st, my_addr);
     issue_k(st);
     issue_scales(st);
@@ -683,6 +686,7 @@ struct ManyTile {
     int n;      // keys that some row may see
     int rank;
     int local;
+    int entry;  // of the table
 };
 
 template <int D, bool FP8, bool SCALED>
@@ -695,9 +699,11 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     __shared__ __attribute__((aligned(1024))) uint8_t lds[S::LDS_BYTES];
     __shared__ __attribute__((aligned(16))) float scales[SCALED ? 2 * S::TILES * 2 * kKeyTile : 4];
     __shared__ float pair_ml[S::PAIR ? kWaves * 64 * 2 : 1];
+    __shared__ int spoiled;  // a value that is not finite was taken out of some tile's V
 
     Item it;
     if (!find_item(a, blockIdx.x, kRowsPerGroup, it)) return;
+    if (threadIdx.x == 0) spoiled = 0;  // (the first tile's barrier comes before any settle_v)
     if (it.head == 0 && it.tile == 0 && it.range == 0 && threadIdx.x == 0 && a.plans) a.plans[it.b] = it.plan;
 
     const int tid = threadIdx.x, lane = tid & 63;
@@ -751,50 +757,65 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     }
 
     // ---- the walk ------------------------------------------------------------------------
-    typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
     const const_i32_ptr table = (const_i32_ptr)(a.pages.table + (table_of(a.pages, it.b) << a.pages.table_shift));
     const int end = min(it.end, walk_tiles(a.pages, most));
+    // the first tile from i on with keys, its page still a table entry to be read
+    // (entry -1: past the last)
     auto tile_from = [&](int i) {
-        ManyTile t{i, -1, 0, 0, 0, 0};
+        ManyTile t{i, -1, 0, 0, 0, 0, -1};
         for (; t.i < end; ++t.i) {
             const uint32_t lt = div((uint32_t)t.i, a.pages.div_pcp);
-            const int rank = t.i - lt * a.pages.pcp, local = lt * kKeyTile;
+            const int rank = t.i - lt * a.pages.pcp, local = lt * kTileKeys;
             const int n = min(owned_of(a.pages, most, rank) - local, kKeyTile);
             const uint32_t blk = div((uint32_t)local, a.pages.div_block);
             if (n <= 0 || (int)blk >= a.pages.max_local_blocks) continue;
-            const int page = table_page(table, rank * a.pages.max_local_blocks + (int)blk, a.pages.table_shift);
-            if ((unsigned)page >= (unsigned)a.pages.num_pages) continue;
             t.n = __builtin_amdgcn_readfirstlane(n);
             t.rank = __builtin_amdgcn_readfirstlane(rank);
             t.local = __builtin_amdgcn_readfirstlane(local);
-            t.page = __builtin_amdgcn_readfirstlane(page);
+            t.entry = __builtin_amdgcn_readfirstlane(rank * a.pages.max_local_blocks + (int)blk);
             t.slot = __builtin_amdgcn_readfirstlane(local - (int)blk * a.pages.block_size);
             break;
         }
         return t;
     };
+    auto read_entry = [&](const ManyTile& t) { return entry_of(table, a.pages, t.entry); };
+    // the tile with its page, from the entry read ahead; tiles without a page are passed over
+    auto with_page = [&](ManyTile t, TableEntry e) {
+        while (t.entry >= 0) {
+            t.page = page_of(a.pages, e);
+            if (t.page >= 0) break;
+            t = tile_from(t.i + 1);
+            e = read_entry(t);
+        }
+        return t;
+    };
+    auto next_tile = [&](int i) {
+        const ManyTile t = tile_from(i);
+        return with_page(t, read_entry(t));
+    };
     FwdArgs f{};
     f.kv = a.pool + it.head * a.pages.head_stride;
     f.head_stride = a.pages.head_stride;
     f.num_kv_heads = a.pages.num_kv_heads;
-    // the thread's scale of tile t: threads 0 .. 63 K's, 64 .. 127 V's (TWO: the
-    // next 128 the second tile's); slots without a token hold none
-    // (opaque here and below: what a thread's index gives is formed where it is used;
-    // kept over the walk it cost Q's registers, parts of which were then read back
-    // from memory for every tile)
-    auto thread = [&]() {
-        int x = tid;
+    // (opaque here and below: what a thread's index or its row gives is formed where
+    // it is used; kept over the walk it cost Q's registers, parts of which were then
+    // read back from memory for every tile)
+    auto opaque = [](int x) {
         asm volatile("" : "+v"(x));
         return x;
     };
+    auto thread = [&]() { return opaque(tid); };
+    auto visible = [&](const ManyTile& t) { return owned_of(a.pages, opaque(seen), t.rank) - t.local; };
+    // the thread's scale of tile t: wave 0 K's, wave 1 V's (TWO: the next two the
+    // second tile's); slots without a token have none
     auto load_scale = [&](const ManyTile& t, const ManyTile& t2) {
-        const int tid = thread();
-        const bool other = TWO && (tid & 128);
+        const bool other = TWO && (wave & 2);
         const int page = other ? t2.page : t.page, slot = other ? t2.slot : t.slot, n = other ? t2.n : t.n;
-        const int key = tid & 63, which = (tid >> 6) & 1;
-        if (page < 0 || key >= n || tid >= 128 * S::TILES) return 0.f;
-        return a.token_scales[(((int64_t)page * 2 + which) * a.pages.num_kv_heads + it.head) * a.pages.block_size + slot +
-                              key];
+        if (page < 0 || wave >= 2 * S::TILES) return 0.f;
+        const float* const of = a.token_scales +
+            (((int64_t)page * 2 + (wave & 1)) * a.pages.num_kv_heads + it.head) * a.pages.block_size + slot;
+        const uint32_t key = thread() & 63;
+        return (int)key < n ? of[key] : 0.f;
     };
 
     SoftmaxState<S> st;
@@ -807,7 +828,6 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     // a row that does not, as 0 times it, unless it is finite.  Rows past the n
     // keys are cleared, and values that are not finite: those join the rows that
     // see their keys after the walk.  Called by the whole workgroup.
-    bool spoiled = false;
     auto settle_v = [&](uint8_t* v, const ManyTile& t) {
         const int tid = thread();
         const int from = max(owned_of(a.pages, least, t.rank) - t.local, 0);
@@ -828,11 +848,13 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
             }
             *at = y;
         }
-        spoiled |= __syncthreads_or(bad) != 0;
+        if (bad) spoiled = 1;
+        __syncthreads();
     };
     auto settled = [&](const ManyTile& t) { return owned_of(a.pages, least, t.rank) - t.local >= kKeyTile; };
 
-    ManyTile cur = tile_from(it.begin), cur2{}, nxt, nxt2{};
+    ManyTile cur = next_tile(it.begin), cur2{}, ahead, ahead2{};
+    TableEntry entry, entry2{};
     float scale = 0.f;
     auto stage = [&](const ManyTile& t, const ManyTile& t2, uint8_t* buf) {
         {
@@ -845,11 +867,22 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
             stage_tile_async<S>(f, TileCursor{0, t2.slot, 0, t2.page * a.pages.page_stride}, buf + 2 * S::TILE, wave, L);
         if constexpr (SCALED) scale = load_scale(t, t2);
     };
-    if constexpr (TWO) cur2 = tile_from(cur.i + 1);
+    if constexpr (TWO) cur2 = next_tile(cur.i + 1);
     stage(cur, cur2, lds);
+    auto look_ahead = [&](int i) {  // (a step ahead of their use: no wait for the table's memory)
+        ahead = tile_from(i);
+        entry = read_entry(ahead);
+        if constexpr (TWO) {
+            ahead2 = tile_from(ahead.i + 1);
+            entry2 = read_entry(ahead2);
+        }
+    };
+    look_ahead((TWO ? cur2.i : cur.i) + 1);
     for (int rbuf = 0; cur.page >= 0; rbuf ^= 1) {
-        nxt = tile_from((TWO ? cur2.i : cur.i) + 1);
-        if constexpr (TWO) nxt2 = tile_from(nxt.i + 1);
+        const ManyTile nxt = with_page(ahead, entry);
+        // (a tile without a page was passed over: the second follows anew)
+        const ManyTile nxt2 = !TWO ? ManyTile{} : nxt.i < ahead2.i ? with_page(ahead2, entry2) : next_tile(nxt.i + 1);
+        look_ahead((TWO ? nxt2.i : nxt.i) + 1);
         const uint32_t rt_off = rbuf * S::BUFFER;
         wait_vmem();  // this wave's loads of the current tiles have landed
         float* const sc = scales + rbuf * S::TILES * 2 * kKeyTile;
@@ -862,11 +895,11 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         if constexpr (TWO) {
             const ManyTile& t = kh ? cur2 : cur;
             if (t.page >= 0)
-                compute_tile<S, 0, true, SCALED>(lds, rt_off + kh * 2 * S::TILE, owned_of(a.pages, seen, t.rank) - t.local,
+                compute_tile<S, 0, true, SCALED>(lds, rt_off + kh * 2 * S::TILE, visible(t),
                                                  qop, a.score_scale, L, hl, st, sc + kh * 2 * kKeyTile);
         } else {
             const int first_key = S::PAIR ? 32 * kh : 0;
-            compute_tile<S, 0, true, SCALED>(lds, rt_off, owned_of(a.pages, seen, cur.rank) - cur.local - first_key, qop,
+            compute_tile<S, 0, true, SCALED>(lds, rt_off, visible(cur) - first_key, qop,
                                              a.score_scale, L, hl, st, sc);
         }
         cur = nxt;
@@ -907,9 +940,10 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         st.m = m;
     }
 
+    if constexpr (!S::PAIR) __syncthreads();  // (spoiled is whole: PAIR has passed two barriers)
     // ---- values that are not finite, for the rows that see them (from the pages) -----------
     if (spoiled) {
-        for (ManyTile t = tile_from(it.begin); t.page >= 0; t = tile_from(t.i + 1)) {
+        for (ManyTile t = next_tile(it.begin); t.page >= 0; t = next_tile(t.i + 1)) {
             const int vis = min(owned_of(a.pages, sees(min(row, rows - 1)), t.rank) - t.local, t.n);
             for (int key = max(owned_of(a.pages, least, t.rank) - t.local, 0); key < t.n; ++key) {
                 const uint8_t* const v = f.kv + t.page * a.pages.page_stride + a.pages.num_kv_heads * a.pages.head_stride +
