@@ -48,7 +48,7 @@ struct Item {
     int begin, end;
     SequencePlan plan;
     Span span;
-    int length;  // of the cache, clamped to what it holds
+    int length;  // of the cache, as given
 };
 
 // Tiles of the walk over positions [0, keys): rank by rank within each 64 local
@@ -59,100 +59,107 @@ __device__ __forceinline__ int walk_tiles(const Pages& p, int keys) {
     return p.pcp * ((most + kTileKeys - 1) / kTileKeys);
 }
 
+// The place of item `at` among the items of its sequence; false for none.
+__device__ __forceinline__ bool place_item(const AttendArgs& a, int at, int walk, Item& it) {
+    const int heads = a.pages.num_kv_heads;
+    if (at < 0) return false;
+    const int rest = at / heads;
+    it.head = at - rest * heads;
+    it.range = rest / it.plan.tiles;
+    // the last rows, which see the most, first
+    it.tile = it.plan.tiles - 1 - (rest - it.range * it.plan.tiles);
+    // (starts that decrease may overflow the sums: no such item)
+    if (it.range >= it.plan.ranges) return false;
+    it.begin = (int)((int64_t)walk * it.range / it.plan.ranges);
+    it.end = (int)((int64_t)walk * (it.range + 1) / it.plan.ranges);
+    return true;
+}
+
 // The item of workgroup `index`; false when there is none.  Every wave of the
-// workgroup finds it by itself, 64 sequences at a time: first the work of the
-// whole chunk, which gives the tiles a range should have so that all ranges
-// fill the GPU once, then the sequence that the index falls into.  (A launch
-// of its own for this took longer than the scan: two dependent loads and a few
-// shuffles for up to 64 sequences.)
+// workgroup finds it by itself (a launch of its own for this took longer), a
+// sequence to a lane: first the work of the whole chunk, which gives the tiles a
+// range should have so that all ranges fill the GPU once, then the sequence that
+// the index falls into.  The first 64 sequences stay in registers (as many as
+// 256, with their loads in flight together, took more of the registers than they
+// saved: seven prompts, D 256, e4m3: 672 -> 702 us).  Sequences of as many rows
+// each whose walks are not cut need no sums (4096 workgroups of one tile each:
+// 300 -> 268 us).
 __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int rows_per_tile, Item& it) {
-    const int lane = threadIdx.x & 63, heads = a.pages.num_kv_heads;
-    auto sequence = [&](int base, Span& span, int& length, int& tiles, int& walk) {
-        span = Span{0, 0};
-        length = tiles = walk = 0;
-        if (base + lane < a.chunk.batch) {
-            span = span_of(a.chunk, base + lane);
-            length = min(max(a.chunk.lengths[base + lane], 0), a.pages.capacity);
-            tiles = (int)(((int64_t)span.count * a.group + rows_per_tile - 1) / rows_per_tile);
-            // (a sequence whose rows see nothing still has an item, for their zeros)
-            walk = max(walk_tiles(a.pages, length), 1);
-        }
+    const int lane = threadIdx.x & 63, heads = a.pages.num_kv_heads, batch = a.chunk.batch;
+    const bool cut = a.part_o != nullptr;
+    auto tiles_of = [&](int count) { return (int)(((int64_t)count * a.group + rows_per_tile - 1) / rows_per_tile); };
+    // (a sequence whose rows see nothing still has an item, for their zeros)
+    auto walk_of = [&](int length) { return max(walk_tiles(a.pages, min(max(length, 0), a.pages.capacity)), 1); };
+    if (!cut && !a.chunk.starts) {
+        const int tiles = tiles_of(a.chunk.each), per = tiles * heads;
+        it.b = index / per;
+        if (it.b >= batch) return false;
+        it.span = span_of(a.chunk, it.b);
+        it.length = a.chunk.lengths[it.b];
+        it.plan = SequencePlan{it.b * per, 1, tiles, rows_per_tile};
+        return place_item(a, index - it.b * per, walk_of(it.length), it);
+    }
+    struct Lane {
+        Span span;
+        int length;
     };
-    Span span, first_span;
-    int length, tiles, walk, first_length, first_tiles, first_walk;
-    // (in 32-bit floats: only the range's length comes of them)
-    float work = 0.f, least = 0.f;
-    for (int base = 0; base < a.chunk.batch; base += 64) {
-        sequence(base, span, length, tiles, walk);
-        if (base == 0) {
-            first_span = span;
-            first_length = length;
-            first_tiles = tiles;
-            first_walk = walk;
-        }
-        work += (float)tiles * (float)walk;
-        least += (float)tiles;
-    }
-    const float slots = (float)a.slots;
-    least = sum_over_lanes<64>(least) * heads;
-    const float share = ceilf(sum_over_lanes<64>(work) * heads / slots);
-    float length_of = fmaxf(fminf(share, 0x1p30f), (float)a.min_range);
-    // Each sequence's last range is a shorter one, so that ranges of the fair
-    // share are more than the GPU holds at once, and the few left over would run
-    // after all others: longer ranges, until all run together.  (64 sequences
-    // of 512 to 8192 tokens, 2 heads at D 256, e4m3: 83.2 -> 74.6 us.)
-    for (int tries = 0; tries < 6 && least < slots; ++tries) {
-        float count = 0.f;
-        for (int base = 0; base < a.chunk.batch; base += 64) {
-            if (base == 0) {
-                tiles = first_tiles;
-                walk = first_walk;
-            } else {
-                sequence(base, span, length, tiles, walk);
+    auto load = [&](int base) {
+        Lane x{{0, 0}, 0};
+        if (base + lane < batch) x = Lane{span_of(a.chunk, base + lane), a.chunk.lengths[base + lane]};
+        return x;
+    };
+    const Lane kept = load(0);
+    const int tiles = tiles_of(kept.span.count), walk = walk_of(kept.length);
+    int range = 1 << 30;  // (beyond any walk)
+    if (cut) {
+        // f(tiles, walk) summed over the sequences (in 32-bit floats: only the
+        // range's length comes of them)
+        auto over_all = [&](auto f) {
+            float sum = f(tiles, walk);
+            for (int base = 64; base < batch; base += 64) {
+                const Lane x = load(base);
+                sum += f(tiles_of(x.span.count), walk_of(x.length));
             }
-            count += (float)(tiles * ((walk + (int)length_of - 1) / (int)length_of));
-        }
-        count = sum_over_lanes<64>(count) * heads;
-        if (count <= slots) break;
-        length_of = fminf(ceilf(fmaxf(length_of + 1.f, length_of * (count / slots))), 0x1p30f);
+            return sum_over_lanes<64>(sum) * heads;
+        };
+        const float slots = (float)a.slots;
+        const float share = ceilf(over_all([](int t, int w) { return (float)t * (float)w; }) / slots);
+        float length_of = fmaxf(fminf(share, 0x1p30f), (float)a.min_range);
+        // Each sequence's last range is a shorter one, so that ranges of the fair
+        // share are more than the GPU holds at once, and the few left over would run
+        // after all others: longer ranges, until all run together.  (64 sequences
+        // of 512 to 8192 tokens, 2 heads at D 256, e4m3: 83.2 -> 74.6 us.)
+        if (over_all([](int t, int) { return (float)t; }) < slots)
+            for (int tries = 0; tries < 6; ++tries) {
+                const int len = (int)length_of;
+                const float count = over_all([&](int t, int w) { return (float)(t * ((w + len - 1) / len)); });
+                if (count <= slots) break;
+                length_of = fminf(ceilf(fmaxf(length_of + 1.f, length_of * (count / slots))), 0x1p30f);
+            }
+        range = __builtin_amdgcn_readfirstlane((int)length_of);
     }
-    const int range = __builtin_amdgcn_readfirstlane((int)length_of);
     int before = 0;
-    for (int base = 0; base < a.chunk.batch; base += 64) {
-        if (base == 0) {
-            span = first_span;
-            length = first_length;
-            tiles = first_tiles;
-            walk = first_walk;
-        } else {
-            sequence(base, span, length, tiles, walk);
-        }
-        const int ranges = (walk + range - 1) / range;
-        const int items = tiles * heads * ranges;
-        const int incl = inclusive_sum(items);
+    bool found = false;
+    auto look = [&](int base, const Lane& x, int t, int w) {
+        const int ranges = (w + range - 1) / range, items = t * heads * ranges, incl = inclusive_sum(items);
         const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > index);
         if (past) {
             const int src = __builtin_ctzll(past);
-            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
+            auto of = [&](int y) { return __builtin_amdgcn_readlane(y, src); };
             it.b = base + src;
-            it.span = Span{of(span.first), of(span.count)};
-            it.length = of(length);
-            it.plan = SequencePlan{before + of(incl) - of(items), of(ranges), of(tiles), rows_per_tile};
-            int at = index - it.plan.first_item;
-            if (at < 0) return false;
-            const int rest = at / heads;
-            it.head = at - rest * heads;
-            it.range = rest / it.plan.tiles;
-            // the last rows, which see the most, first
-            it.tile = it.plan.tiles - 1 - (rest - it.range * it.plan.tiles);
-            // (starts that decrease may overflow the sums: no such item)
-            if (it.range >= it.plan.ranges) return false;
-            const int w = of(walk);
-            it.begin = (int)((int64_t)w * it.range / it.plan.ranges);
-            it.end = (int)((int64_t)w * (it.range + 1) / it.plan.ranges);
+            it.span = Span{of(x.span.first), of(x.span.count)};
+            it.length = of(x.length);
+            it.plan = SequencePlan{before + of(incl) - of(items), of(ranges), of(t), rows_per_tile};
+            found = place_item(a, index - it.plan.first_item, of(w), it);
             return true;
         }
         before += __builtin_amdgcn_readlane(incl, 63);
+        return false;
+    };
+    if (look(0, kept, tiles, walk)) return found;
+    for (int base = 64; base < batch; base += 64) {
+        const Lane x = load(base);
+        if (look(base, x, tiles_of(x.span.count), walk_of(x.length))) return found;
     }
     return false;
 }
@@ -274,9 +281,8 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     const int row0 = it.tile * S::ROWS;
     // the tile's last row sees the most
     const int last = min(row0 + S::ROWS, rows) - 1;
-    const int64_t len = a.chunk.lengths[it.b];
     auto sees = [&](int row) {
-        const int64_t np = len - it.span.count + row / a.group + 1;
+        const int64_t np = (int64_t)it.length - it.span.count + row / a.group + 1;
         return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
     };
     const int most = __builtin_amdgcn_readfirstlane(sees(last)), least = __builtin_amdgcn_readfirstlane(sees(row0));
@@ -716,9 +722,8 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     const int rows = it.span.count * a.group, row0 = it.tile * kRowsPerGroup;
     // (rows past the last do as the last, unseen)
     const int row_c = min(row0 + pw * kRowsPerWave + j, rows - 1);
-    const int64_t len = a.chunk.lengths[it.b];
     auto sees = [&](int r) {
-        const int64_t np = len - it.span.count + r / a.group + 1;
+        const int64_t np = (int64_t)it.length - it.span.count + r / a.group + 1;
         return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
     };
     auto index_of = [&](int r) {
@@ -906,6 +911,11 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         cur2 = nxt2;
     }
 
+    // (the arguments are read anew: kept over the walk they cost it scalar
+    // registers; seven prompts, D 256, e4m3: 696 -> 682 us)
+    auto* args = (const __attribute__((address_space(4))) uint8_t*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    const AttendArgs& z = *(const AttendArgs*)args;
     const int lane2 = thread() & 63, h2 = lane2 >> 5;
     const int row = row0 + pw * kRowsPerWave + (lane2 & 31);
 
@@ -970,14 +980,15 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     // ---- O = O^T / l, or the range's partial result ---------------------------------------
     const float total = halves_sum(st.l);
     const bool empty = total == 0.f;
-    const float inv = empty ? 0.f : a.v_scale / total;
+    const float inv = empty ? 0.f : z.v_scale / total;
     const float log2sum = empty ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
     if (row >= rows) return;
-    const int64_t row_index = index_of(row);
+    const int64_t row_index =
+        (int64_t)(it.span.first + row / z.group) * z.num_q_heads + it.head * z.group + row % z.group;
     const bool part = it.plan.ranges > 1;
     const int64_t prow = (int64_t)blockIdx.x * kRowsPerGroup + pw * kRowsPerWave + (lane2 & 31);
-    float* const po = a.part_o + prow * D;
-    uint8_t* const orow = a.out + row_index * D * 2;
+    float* const po = z.part_o + prow * D;
+    uint8_t* const orow = z.out + row_index * D * 2;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1001,9 +1012,9 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         }
     if (h2 == 0) {
         if (part)
-            a.part_lse[prow] = log2sum;
-        else if (a.lse)
-            a.lse[row_index] = log2sum * kLn2;
+            z.part_lse[prow] = log2sum;
+        else if (z.lse)
+            z.lse[row_index] = log2sum * kLn2;
     }
 }
 
@@ -1092,7 +1103,8 @@ __global__ void __launch_bounds__(256) merge_few_ranges_kernel(AttendArgs a) {
 
 // Rows with many ranges: a workgroup of 16 waves per 64 values of a (row, Q
 // head), 64 partials at a time, 16 lanes to each; the four of a wave meet in
-// registers, the waves in LDS.  (32 rows of 256 ranges at D 256: MERGEFIG.)
+// registers, the waves in LDS.  (32 rows of 256 ranges at D 256:
+// 5.1 us; 9.0 with one wave for a row.)
 constexpr int kMergeParts = 64;  // values of a workgroup
 template <int D>
 __global__ void __launch_bounds__(1024) merge_many_ranges_kernel(AttendArgs a) {

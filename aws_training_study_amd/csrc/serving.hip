@@ -172,9 +172,14 @@ int32_t write_chunk(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary
 
 // ---- attention ---------------------------------------------------------------
 
+// A range of a walk has at least this many tiles (64 keys each).  Few rows: one
+// token over 1024 to 8192 keys at D 256 took 16.4 us a call with 8, 14.5 with 4,
+// 12.6 to 13.9 with 2; many: a range's start costs several tiles' time.
+constexpr int kMinRangeFew = 2, kMinRangeMany = 8;
+
 struct AttendKernel {
     const void* fn;
-    int threads, rows, per_cu;
+    int threads, rows, per_cu, min_range;
 };
 // (a kernel with and without token scales has the same shape)
 template <int D, bool FP8, int RT>
@@ -182,7 +187,7 @@ AttendKernel few_kernel(bool scaled) {
     using S = FewShape<D, FP8, RT>;
     return AttendKernel{scaled ? (const void*)attend_few_kernel<D, FP8, FP8, RT>
                                : (const void*)attend_few_kernel<D, FP8, false, RT>,
-                        S::THREADS, S::ROWS, S::PER_CU};
+                        S::THREADS, S::ROWS, S::PER_CU, kMinRangeFew};
 }
 template <bool FP8, int RT>
 AttendKernel few_kernel_for(int d, bool scaled) {
@@ -196,15 +201,12 @@ AttendKernel many_kernel(bool scaled) {
     using S = TileShape<D, FP8, false>;
     return AttendKernel{scaled ? (const void*)attend_many_kernel<D, FP8, FP8>
                                : (const void*)attend_many_kernel<D, FP8, false>,
-                        S::THREADS, kRowsPerGroup, S::PAIR ? 1 : 2};
+                        S::THREADS, kRowsPerGroup, S::PAIR ? 1 : 2, kMinRangeMany};
 }
 template <bool FP8>
 AttendKernel many_kernel_for(int d, bool scaled) {
     return d == 64 ? many_kernel<64, FP8>(scaled) : d == 128 ? many_kernel<128, FP8>(scaled) : many_kernel<256, FP8>(scaled);
 }
-
-// A range of a walk has at least this many tiles (64 keys each).
-constexpr int kMinRange = 8;
 
 struct AttendPlan {
     AttendKernel kernel;
@@ -268,7 +270,7 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     a.group = p->num_q_heads / p->num_kv_heads;
     a.max_items = (int32_t)w.items;
     a.slots = kCUs * w.kernel.per_cu;
-    a.min_range = w.ranges ? kMinRange : 1 << 30;  // (beyond any walk)
+    a.min_range = w.kernel.min_range;
     a.score_scale = p->softmax_scale * p->k_scale * kLog2e;
     a.v_scale = p->v_scale;
     if (w.ranges) {
