@@ -9,8 +9,13 @@ namespace pcpa {
 namespace chunk {
 
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
 constexpr int kTileKeys = 64;  // keys of a walk's tile: a whole number of them to a page
+
+// The maximum before any score: finite, as keys may be hidden from a row before
+// any that is not (2^(-inf - kNoScore) is 0), and no more than any finite score.
+constexpr float kNoScore = -0x1.fffffep127f;
 
 // What the merge needs to find a sequence's partial results: written by the
 // sequence's first workgroup.
@@ -18,7 +23,6 @@ struct SequencePlan {
     int32_t first_item;  // of all its (range, row tile from the last on, KV head) items, KV head fastest
     int32_t ranges;      // its walk is cut into; 1: results are final
     int32_t tiles;       // row tiles
-    int32_t rows;        // rows of a row tile
 };
 
 struct AttendArgs {
@@ -31,13 +35,15 @@ struct AttendArgs {
     float* lse;
     int32_t num_q_heads;
     int32_t group;
+    int32_t rows;          // of a workgroup's row tile
     int32_t max_items;     // the launch's workgroups
     int32_t slots;         // workgroups that the GPU holds at once
     int32_t min_range;     // tiles a range has at least
     float score_scale;     // softmax_scale * k_scale * log2(e)
     float v_scale;
     float* part_o;         // [max_items, rows, D] fp32 normalised outputs of ranges
-    float* part_lse;       // [max_items, rows] log2 of their sums
+    v2f* part_ml;          // [max_items, rows] their maxima and sums (one log of both would round
+                           // the sum away where scores are large)
     SequencePlan* plans;   // [batch]
 };
 
@@ -96,7 +102,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
         if (it.b >= batch) return false;
         it.span = span_of(a.chunk, it.b);
         it.length = a.chunk.lengths[it.b];
-        it.plan = SequencePlan{it.b * per, 1, tiles, rows_per_tile};
+        it.plan = SequencePlan{it.b * per, 1, tiles};
         return place_item(a, index - it.b * per, walk_of(it.length), it);
     }
     struct Lane {
@@ -149,7 +155,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
             it.b = base + src;
             it.span = Span{of(x.span.first), of(x.span.count)};
             it.length = of(x.length);
-            it.plan = SequencePlan{before + of(incl) - of(items), of(ranges), of(t), rows_per_tile};
+            it.plan = SequencePlan{before + of(incl) - of(items), of(ranges), of(t)};
             found = place_item(a, index - it.plan.first_item, of(w), it);
             return true;
         }
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     v4f o[RT][DT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -1.0e30f;  // (finite: a step may be hidden from a row before any that is not)
+        m[rt] = kNoScore;
         l[rt] = 0.f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[rt][dt] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -659,7 +665,7 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
             if (it.plan.ranges > 1) {
                 const int64_t prow = (int64_t)blockIdx.x * S::ROWS + 16 * rt + j;
                 *(v4f*)(a.part_o + prow * D + 4 * c) = empty ? v4f{0.f, 0.f, 0.f, 0.f} : acc * inv;
-                if (c == 0) a.part_lse[prow] = log2sum;
+                if (c == 0) a.part_ml[prow] = v2f{top, total};
             } else {
                 const int tok = it.span.first + row / a.group, hd = it.head * a.group + row % a.group;
                 const int64_t at = (int64_t)tok * a.num_q_heads + hd;
@@ -824,7 +830,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     };
 
     SoftmaxState<S> st;
-    st.m = -1.0e30f;  // (finite: a tile may be hidden from a row before any that is not)
+    st.m = kNoScore;
     st.l = 0.f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) st.o[dt] = v16f{};
@@ -1012,7 +1018,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         }
     if (h2 == 0) {
         if (part)
-            z.part_lse[prow] = log2sum;
+            z.part_ml[prow] = v2f{st.m, total};
         else if (z.lse)
             z.lse[row_index] = log2sum * kLn2;
     }
@@ -1030,28 +1036,30 @@ struct Partials {
 __device__ __forceinline__ bool partials_of(const AttendArgs& a, int b, int token, int head, Partials& p) {
     if (b < 0) return false;
     const SequencePlan plan = a.plans[b];
-    if (plan.ranges <= 1 || plan.rows <= 0) return false;
+    if (plan.ranges <= 1) return false;
     const Span span = span_of(a.chunk, b);
     const int kv = head / a.group;
     const int row = (token - span.first) * a.group + (head - kv * a.group);
-    const int tile = row / plan.rows;
-    const int64_t heads = a.pages.num_kv_heads, item = plan.first_item + (plan.tiles - 1 - tile) * heads + kv;
+    const int tile = row / a.rows;
+    const int64_t heads = a.pages.num_kv_heads, item = plan.first_item + ((int64_t)plan.tiles - 1 - tile) * heads + kv;
     const int64_t step = plan.tiles * heads;
-    // (only starts that decrease lead past the launch's items)
-    if (plan.first_item < 0 || tile >= plan.tiles || item + (plan.ranges - 1) * step >= a.max_items) return false;
-    p = Partials{item * plan.rows + row % plan.rows, step * plan.rows, plan.ranges};
+    // (only with starts that decrease is there a plan that no workgroup wrote:
+    // whatever it holds, nothing past the launch's items is read)
+    if (plan.first_item < 0 || tile >= plan.tiles || step > a.max_items || plan.ranges > a.max_items ||
+        item + (plan.ranges - 1) * step >= a.max_items)
+        return false;
+    p = Partials{item * a.rows + row % a.rows, step * a.rows, plan.ranges};
     return true;
 }
 
-// The running merge of partial results: weights 2^(log2 sum - top).
+// The running merge of partial results: weights sum 2^(max - top).
 struct Merged {
     float top, total;
     v4f acc;
-    __device__ __forceinline__ void add(float log2sum, const v4f& x) {
-        if (log2sum == -INFINITY) return;  // nothing seen in it
-        const float next = fmaxf(top, log2sum);
-        const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
-        const float weight = __builtin_amdgcn_exp2f(log2sum - next);
+    __device__ __forceinline__ void add(const v2f& ml, const v4f& x) {
+        const float next = fmaxf(top, ml[0]);
+        const float keep = __builtin_amdgcn_exp2f(top - next);
+        const float weight = ml[1] * __builtin_amdgcn_exp2f(ml[0] - next);
         total = fmaf(total, keep, weight);
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] = fmaf(acc[k], keep, weight * x[k]);
@@ -1084,18 +1092,18 @@ __global__ void __launch_bounds__(256) merge_few_ranges_kernel(AttendArgs a) {
     for (int head = blockIdx.y * AT_ONCE + threadIdx.x / LANES; head < a.num_q_heads; head += gridDim.y * AT_ONCE) {
         Partials p;
         if (!partials_of(a, b, token, head, p)) continue;
-        Merged r{-INFINITY, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
+        Merged r{kNoScore, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
         for (int s0 = 0; s0 < p.ranges; s0 += UNROLL) {
-            float ls[UNROLL];
+            v2f ml[UNROLL];
             v4f x[UNROLL];
 #pragma unroll
             for (int u = 0; u < UNROLL; ++u) {
                 const int64_t row = p.first + min(s0 + u, p.ranges - 1) * p.step;
-                ls[u] = a.part_lse[row];
+                ml[u] = a.part_ml[row];
                 x[u] = *(const v4f*)(a.part_o + row * D + 4 * c);
             }
 #pragma unroll
-            for (int u = 0; u < UNROLL; ++u) r.add(s0 + u < p.ranges ? ls[u] : -INFINITY, x[u]);
+            for (int u = 0; u < UNROLL; ++u) r.add(s0 + u < p.ranges ? ml[u] : v2f{kNoScore, 0.f}, x[u]);
         }
         store_merged<D>(a, (int64_t)token * a.num_q_heads + head, c, r.top, r.total, r.acc);
     }
@@ -1117,22 +1125,22 @@ __global__ void __launch_bounds__(1024) merge_many_ranges_kernel(AttendArgs a) {
     if (!partials_of(a, b, token, head, p)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, at = threadIdx.x / LANES, c = threadIdx.x % LANES;
     const int value = blockIdx.z * kMergeParts + 4 * c;
-    Merged r{-INFINITY, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
+    Merged r{kNoScore, 0.f, v4f{0.f, 0.f, 0.f, 0.f}};
     for (int s0 = at; s0 < p.ranges; s0 += AT_ONCE * UNROLL) {
-        float ls[UNROLL];
+        v2f ml[UNROLL];
         v4f x[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const int64_t row = p.first + min(s0 + u * AT_ONCE, p.ranges - 1) * p.step;
-            ls[u] = a.part_lse[row];
+            ml[u] = a.part_ml[row];
             x[u] = *(const v4f*)(a.part_o + row * D + value);
         }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) r.add(s0 + u * AT_ONCE < p.ranges ? ls[u] : -INFINITY, x[u]);
+        for (int u = 0; u < UNROLL; ++u) r.add(s0 + u * AT_ONCE < p.ranges ? ml[u] : v2f{kNoScore, 0.f}, x[u]);
     }
-    // (a partial that saw nothing weighs nothing; one that is NaN has a NaN total)
+    // (a partial that saw nothing has the sum 0; one that is NaN has a NaN sum)
     float top = quarters_max(r.top);
-    float weight = r.total == 0.f ? 0.f : __builtin_amdgcn_exp2f(r.top - top);
+    float weight = __builtin_amdgcn_exp2f(r.top - top);
     float total = quarters_sum(weight * r.total);
     v4f acc;
 #pragma unroll
@@ -1151,7 +1159,7 @@ __global__ void __launch_bounds__(1024) merge_many_ranges_kernel(AttendArgs a) {
     acc = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-        weight = part_ml[i][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(part_ml[i][0] - top);
+        weight = __builtin_amdgcn_exp2f(part_ml[i][0] - top);
         total = fmaf(weight, part_ml[i][1], total);
         const v4f x = part[i][c];
 #pragma unroll

@@ -110,6 +110,7 @@ struct Call {
     struct Space {
         void* stream;
         at::Tensor tensor;
+        unsigned long thread = 0;  // (attention of a chunk)
     };
     std::vector<Space>* spaces;
     // rotation
@@ -322,6 +323,21 @@ pcpa_rows view_of(const at::Tensor& t) {
     return pcpa_rows{t.data_ptr(), t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
 }
 
+// Whether the memory that the rows of a and b lie in meets (what is in between is
+// the general path's to look at).
+bool meet(const at::Tensor& a, const at::Tensor& b) {
+    auto end = [](const at::Tensor& t) {
+        int64_t last = 0;
+        for (int i = 0; i < 3; ++i) last += (t.size(i) - 1) * t.stride(i);
+        return (const char*)t.data_ptr() + 2 * (last + 1);
+    };
+    return (const char*)a.data_ptr() < end(b) && (const char*)b.data_ptr() < end(a);
+}
+// Whether a given output is its own input, or apart from it.
+bool in_place_or_apart(const at::Tensor& out, const at::Tensor& in) {
+    return (out.data_ptr() == in.data_ptr() && out.strides() == in.strides()) || !meet(out, in);
+}
+
 // The chunk of `n` rows that lengths and starts describe.
 bool chunk_of(const Call* c, const at::Tensor& lengths, const at::Tensor* starts, int64_t n, int dev, pcpa_chunk& out) {
     if (!on_gpu(lengths, at::kInt, dev) || lengths.dim() != 1 || lengths.size(0) < 1 || lengths.size(0) >= INT32_MAX)
@@ -363,6 +379,7 @@ bool rotary_of(const Call* c, const at::Tensor& turns, const at::Tensor* qw, con
         if (!w) continue;
         const bool f32 = w->scalar_type() == at::kFloat;
         if (!on_gpu(*w, f32 ? at::kFloat : at::kBFloat16, dev) || !shaped(*w, {c->p.head_dim})) return false;
+        if ((uintptr_t)w->data_ptr() & (f32 ? 15u : 7u)) return false;
         r.weight_dtype = f32 ? PCPA_DTYPE_FP32 : PCPA_DTYPE_BF16;
     }
     if (qw && kw && qw->scalar_type() != kw->scalar_type()) return false;
@@ -412,6 +429,8 @@ PyObject* rotate(Call* c, PyObject* const* a) {
     if (!rotary_of(c, *turns, qw, kw, dev, r) || !output(a[7], *q, {n, p.num_q_heads, p.head_dim}, dev, q_out) ||
         !output(a[8], *q, {n, p.num_kv_heads, p.head_dim}, dev, k_out))
         GIVE_UP;
+    if (a[7] != Py_None && (!in_place_or_apart(q_out, *q) || meet(q_out, *k) || meet(q_out, k_out))) GIVE_UP;
+    if (a[8] != Py_None && (!in_place_or_apart(k_out, *k) || meet(k_out, *q) || meet(k_out, q_out))) GIVE_UP;
     void* stream = nullptr;
     if (!current_stream(dev, stream)) GIVE_UP;
     const pcpa_rows qi = view_of(*q), ki = view_of(*k), qo = view_of(q_out), ko = view_of(k_out);
@@ -499,6 +518,7 @@ PyObject* chunk_prepare(Call* c, PyObject* const* a) {
         !cache_of(c, *kv, *table, scales, a[9], a[10], chunk.batch, dev, p) || !rotary_of(c, *turns, qw, kw, dev, r) ||
         !output(a[12], *q, {n, p.num_q_heads, p.head_dim}, dev, q_out))
         GIVE_UP;
+    if (a[12] != Py_None && (!in_place_or_apart(q_out, *q) || meet(q_out, *k) || meet(q_out, *v))) GIVE_UP;
     void* stream = nullptr;
     if (!current_stream(dev, stream)) GIVE_UP;
     const pcpa_rows qi = view_of(*q), ki = view_of(*k), vi = view_of(*v), qo = view_of(q_out);
@@ -533,7 +553,9 @@ PyObject* cache_read(Call* c, PyObject* const* a) {
     return tensors(k, v);
 }
 
-// The workspace of `bytes` kept for `stream`; one of the graph's own under capture.
+// The workspace of `bytes` kept for this thread's calls on `stream` (another
+// thread's launches may come between a call's two); one of the graph's own under
+// capture.
 bool chunk_workspace(Call* c, int64_t bytes, void* stream, const at::Tensor& q, at::Tensor& hold) {
     PyObject* capturing = PyObject_CallNoArgs(g_capturing);
     const int is = capturing ? PyObject_IsTrue(capturing) : -1;
@@ -543,8 +565,9 @@ bool chunk_workspace(Call* c, int64_t bytes, void* stream, const at::Tensor& q, 
         hold = at::empty({bytes}, q.options().dtype(at::kByte).requires_grad(false));
         return true;
     }
+    const unsigned long thread = PyThread_get_thread_ident();
     for (const Call::Space& s : *c->spaces)
-        if (s.stream == stream && s.tensor.get_device() == q.get_device()) {
+        if (s.stream == stream && s.thread == thread && s.tensor.get_device() == q.get_device()) {
             if (s.tensor.numel() >= bytes) {
                 hold = s.tensor;
                 return true;
@@ -557,7 +580,7 @@ bool chunk_workspace(Call* c, int64_t bytes, void* stream, const at::Tensor& q, 
     if (!t) return false;
     hold = THPVariable_Unpack(t);
     Py_DECREF(t);
-    c->spaces->push_back({stream, hold});
+    c->spaces->push_back({stream, hold, thread});
     return true;
 }
 
@@ -577,7 +600,7 @@ PyObject* chunk_attention(Call* c, PyObject* const* a) {
     if (!on_gpu(*q, at::kBFloat16, dev) || !shaped(*q, {n, p.num_q_heads, p.head_dim}) ||
         ((uintptr_t)q->data_ptr() & 15u) || !chunk_of(c, *lengths, starts, n, dev, chunk) ||
         !cache_of(c, *kv, *table, scales, a[5], a[6], chunk.batch, dev, p) ||
-        (given_ws && !on_gpu(*given_ws, at::kByte, dev)) || !output(a[8], *q, q->sizes(), dev, out))
+        (given_ws && !on_gpu(*given_ws, at::kByte, dev)) || !output(a[8], *q, q->sizes(), dev, out) || (a[8] != Py_None && !in_place_or_apart(out, *q)))
         GIVE_UP;
     void* stream = nullptr;
     if (!current_stream(dev, stream)) GIVE_UP;

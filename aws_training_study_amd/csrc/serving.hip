@@ -22,10 +22,13 @@ int32_t check_chunk(const pcpa_params* p, const pcpa_chunk* c) {
     const int64_t capacity = (int64_t)p->pcp_size * p->max_local_blocks * p->block_size;
     // (256: room for the walk's rounding up)
     if (capacity > INT32_MAX - 256ll * p->pcp_size || (int64_t)p->pcp_size * c->interleave > INT32_MAX ||
-        (int64_t)c->num_tokens * p->num_q_heads > INT32_MAX)
+        (int64_t)c->num_tokens * p->num_q_heads > INT32_MAX - 256)  // (256: a last row tile's)
         return PCPA_ERR_TOO_LARGE;
     return PCPA_OK;
 }
+
+// A launch has fewer than 2^32 threads.
+bool too_many(int64_t blocks, int threads) { return blocks > (int64_t)(UINT32_MAX / threads); }
 
 // The pages of a launch; the table holds `batch` sequences.
 int32_t check_pages(const pcpa_params* p, const void* block_table, const void* kv_pages, const float* token_scales) {
@@ -69,11 +72,14 @@ bool misaligned(const pcpa_rows* r) {
 RowsIn rows_in(const pcpa_rows* r) { return RowsIn{(const uint8_t*)r->data, r->token_stride * 2, r->head_stride * 2}; }
 RowsOut rows_out(const pcpa_rows* r) { return RowsOut{(uint8_t*)r->data, r->token_stride * 2, r->head_stride * 2}; }
 
+// The square root's reciprocal takes no smaller numbers.
+constexpr float kLeastEps = 0x1p-126f;
+
 int32_t check_rotary(const pcpa_params* p, const pcpa_rotary* r) {
     if (!r) return PCPA_ERR_NULL_POINTER;
     if (r->rotary_dim < 0 || r->rotary_dim > p->head_dim || r->rotary_dim % 16) return PCPA_ERR_BAD_SHAPE;
     if (r->rotary_dim > 0 && !r->turns) return PCPA_ERR_NULL_POINTER;
-    if (!isfinite(r->amplitude) || !isfinite(r->norm_eps) || r->norm_eps < 0.f) return PCPA_ERR_BAD_SCALE;
+    if (!isfinite(r->amplitude) || !isfinite(r->norm_eps) || !(r->norm_eps >= kLeastEps)) return PCPA_ERR_BAD_SCALE;
     const bool f32 = r->weight_dtype == PCPA_DTYPE_FP32;
     if (!f32 && r->weight_dtype != PCPA_DTYPE_BF16) return PCPA_ERR_BAD_DTYPE;
     if (((uintptr_t)r->q_weight | (uintptr_t)r->k_weight) & (f32 ? 15u : 7u)) return PCPA_ERR_MISALIGNED;
@@ -122,7 +128,7 @@ int32_t launch_tokens(TokenArgs& a, const pcpa_params* p, hipStream_t stream) {
     const int64_t q_parts = (q_groups + ng - 1) / ng, blocks_of_tokens = (n + ng - 1) / ng;
     const int64_t q_waves = n * q_parts, kv_waves = blocks_of_tokens * kv_groups;
     const int64_t waves = q_waves + kinds * kv_waves, per = kTokenThreads / 64, blocks = (waves + per - 1) / per;
-    if (waves > INT32_MAX - per) return PCPA_ERR_TOO_LARGE;
+    if (waves > INT32_MAX - per || too_many(blocks, kTokenThreads)) return PCPA_ERR_TOO_LARGE;
     a.waves = (int32_t)waves;
     a.q_waves = (int32_t)q_waves;
     a.q_parts = (int32_t)q_parts;
@@ -212,7 +218,7 @@ struct AttendPlan {
     AttendKernel kernel;
     int64_t items;        // workgroups of the launch
     bool ranges;          // walks may be cut into ranges
-    int64_t part_lse, plans, bytes;
+    int64_t part_ml, plans, bytes;
 };
 
 AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = false) {
@@ -230,11 +236,13 @@ AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = 
     const int64_t tiles = c->num_tokens * group / w.kernel.rows + sequences;
     const int64_t slots = (int64_t)kCUs * w.kernel.per_cu;
     w.ranges = c->num_tokens > 0 && tiles * p->num_kv_heads < 4 * slots;
-    w.items = tiles * p->num_kv_heads + (w.ranges ? slots : 0);
+    // (the device sums the work in 32-bit floats, which may be less by 2^-24 for each
+    // of a lane's sequences)
+    w.items = tiles * p->num_kv_heads + (w.ranges ? slots + slots / 64 : 0);
     if (w.ranges) {
         const int64_t rows = w.items * w.kernel.rows;
-        w.part_lse = rows * d * 4;
-        w.plans = w.part_lse + rows * 4;
+        w.part_ml = rows * d * 4;
+        w.plans = w.part_ml + rows * 8;
         w.bytes = w.plans + (int64_t)c->batch * sizeof(SequencePlan);
     }
     return w;
@@ -256,7 +264,7 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     if ((uintptr_t)lse & 3u) return PCPA_ERR_MISALIGNED;
     const AttendPlan w = attend_plan(p, c, token_scales != nullptr);
     if (workspace_bytes < 0 || (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes))) return PCPA_ERR_WORKSPACE;
-    if (p->num_q_heads > 65535 || w.items > INT32_MAX / 64) return PCPA_ERR_TOO_LARGE;
+    if (p->num_q_heads > 65535 || too_many(w.items, w.kernel.threads)) return PCPA_ERR_TOO_LARGE;
     if (c->num_tokens == 0) return PCPA_OK;
     AttendArgs a{};
     a.chunk = desc_of(c);
@@ -268,6 +276,7 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     a.lse = lse;
     a.num_q_heads = p->num_q_heads;
     a.group = p->num_q_heads / p->num_kv_heads;
+    a.rows = w.kernel.rows;
     a.max_items = (int32_t)w.items;
     a.slots = kCUs * w.kernel.per_cu;
     a.min_range = w.kernel.min_range;
@@ -275,7 +284,7 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     a.v_scale = p->v_scale;
     if (w.ranges) {
         a.part_o = (float*)workspace;
-        a.part_lse = (float*)((uint8_t*)workspace + w.part_lse);
+        a.part_ml = (v2f*)((uint8_t*)workspace + w.part_ml);
         a.plans = (SequencePlan*)((uint8_t*)workspace + w.plans);
     }
     void* args[] = {&a};
@@ -384,7 +393,7 @@ int32_t pcpa_cache_read(const pcpa_params* p, int32_t interleave, int64_t first_
     const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
     const ReadKernel kernel = fp8 ? read_kernel_for<true>(p->head_dim) : read_kernel_for<false>(p->head_dim);
     const int64_t blocks = ((int64_t)num_tokens + kernel.tokens - 1) / kernel.tokens;
-    if (p->num_kv_heads > 65535) return PCPA_ERR_TOO_LARGE;
+    if (p->num_kv_heads > 65535 || too_many(blocks, kTokenThreads)) return PCPA_ERR_TOO_LARGE;
     void* args[] = {&a};
     return hipLaunchKernel(kernel.fn, dim3((unsigned)blocks, p->num_kv_heads, 2), dim3(kTokenThreads), args, 0,
                            (hipStream_t)stream) == hipSuccess

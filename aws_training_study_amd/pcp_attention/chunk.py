@@ -29,7 +29,16 @@ from typing import Optional
 
 from .config import PCPAttentionConfig
 from .kernel import _KV_DTYPE_CODES, _torch_kv_dtype
-from .rotary import QueryKeyRotation, RotaryEmbedding, _check_lengths, _own_places, _pointer, _row_view, _rows
+from .rotary import (
+    QueryKeyRotation,
+    RotaryEmbedding,
+    _check_lengths,
+    _check_output,
+    _own_places,
+    _pointer,
+    _row_view,
+    _rows,
+)
 
 
 def empty_token_scales(config: PCPAttentionConfig, device, num_pages: Optional[int] = None):
@@ -123,8 +132,9 @@ class ChunkCacheWriter(_CacheOperator):
     the pages (values that are not finite become NaN codes); without, the given
     ``k_scale``/``v_scale`` hold for all, as in ``KVCacheWriter``.  A BF16 pool
     holds x.  Rows whose position is negative or beyond the cache, or whose
-    table entry is outside ``[0, num_pages)``, are not written.  Asynchronous
-    on the current stream.
+    table entry is outside ``[0, num_pages)``, are not written; of two rows for
+    one place (a page that two sequences name for new tokens) either may stay.
+    Asynchronous on the current stream.
     """
 
     def __call__(self, k, v, kv_pages, block_table, lengths, *, chunk_starts=None, k_scale: float = 1.0,
@@ -211,13 +221,14 @@ class ChunkAttentionKernel(_CacheOperator):
     * ``q``: contiguous BF16 ``[n, Hq, D]``; the row at position p of a sequence
       sees the keys at positions ``0 .. p`` of its cache, which already holds the
       chunk's own (``ChunkCacheWriter``).
-    * ``out``: as ``q``; rows of no sequence are left as they are.  A row that
-      sees no key (more new tokens than the cache holds, no page) is zeros.
+    * ``out``: as ``q``, which it may be; rows of no sequence are left as they
+      are.  A row that sees no key (more new tokens than the cache holds, no page)
+      is zeros, as is one whose scores are all ``-inf``.
     * ``return_lse``: also the log-sum-exp of each row's scores, float32 ``[n,
       Hq]``, ``-inf`` for a row that sees no key.
     * ``workspace``: uint8 GPU tensor of ``workspace_bytes(n, batch)`` bytes for
       the partial results of long walks, else one that the object keeps per
-      (device, stream).
+      (device, stream, thread).
 
     Both products run on BF16 operands whatever the cache holds: e4m3 codes are
     widened exactly, the scales applied in float32.  Asynchronous on the current
@@ -247,14 +258,17 @@ class ChunkAttentionKernel(_CacheOperator):
         return size
 
     def _workspace(self, size: int, device, stream: int):
-        """The workspace kept for calls on (``device``, ``stream``), which run in
-        order; a call that is being captured gets one of its graph's memory, as
-        graphs captured on one stream may be replayed on several."""
+        """The workspace kept for this thread's calls on (``device``, ``stream``), which
+        run in order (another thread's launches may come between a call's two); a
+        call that is being captured gets one of its graph's memory, as graphs
+        captured on one stream may be replayed on several."""
+        import threading
+
         import torch
 
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(size, dtype=torch.uint8, device=device)
-        key = (device, stream)
+        key = (device, stream, threading.get_ident())
         ws = self._workspaces.get(key)
         if ws is None or ws.numel() < size:
             if ws is None and len(self._workspaces) >= 16:
@@ -302,6 +316,7 @@ class ChunkAttentionKernel(_CacheOperator):
             _rows("out", out, cfg.num_q_heads, cfg.head_dim, n, device)
             if not out.is_contiguous():
                 raise ValueError(f"out must be contiguous, got strides {tuple(out.stride())}")
+            _check_output("out", out, q)
         lse = torch.empty((n, cfg.num_q_heads), dtype=torch.float32, device=device) if return_lse else None
         if n > 0:
             size = self.workspace_bytes(n, batch, chunk_starts is not None)
@@ -389,6 +404,7 @@ class ChunkStep:
         else:
             _rows("q_out", q_out, cfg.num_q_heads, cfg.head_dim, n, device)
             _own_places("q_out", q_out)
+            _check_output("q_out", q_out, q, k, v)
         rotary = self.rotation._rotary_args(device, q_weight, k_weight)
         if n == 0:
             return q_out

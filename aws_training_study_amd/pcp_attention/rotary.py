@@ -123,6 +123,31 @@ def _own_places(name: str, t) -> None:
         extent = stride * (size - 1) + extent
 
 
+def _share_memory(a, b) -> bool:
+    """Whether rows of ``a`` and ``b`` ``[n, heads, D]`` have memory in common; views of one token stride
+    (parts of one projection's output) are told apart by their places in a token."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    size = a.element_size()
+    (at_a, one_a), (at_b, one_b) = ((t.data_ptr() // size, (t.shape[1] - 1) * t.stride(1) + t.shape[2]) for t in (a, b))
+    n = a.shape[0]
+    if at_a >= at_b + (n - 1) * b.stride(0) + one_b or at_b >= at_a + (n - 1) * a.stride(0) + one_a:
+        return False
+    step = a.stride(0)
+    if n > 1 and step == b.stride(0) and step > 0:
+        apart = (at_b - at_a) % step
+        return apart < one_a or apart + one_b > step
+    return True
+
+
+def _check_output(name: str, out, own, *others) -> None:
+    """``ValueError`` unless ``out`` is its own input ``own`` or shares no memory with any."""
+    same = out.data_ptr() == own.data_ptr() and all(
+        s == t for n, s, t in zip(own.shape, out.stride(), own.stride()) if n > 1)
+    if (not same and _share_memory(out, own)) or any(_share_memory(out, t) for t in others):
+        raise ValueError(f"{name} must be its own input or share no memory with any")
+
+
 def _check_lengths(lengths, chunk_starts, batch: Optional[int], num_tokens: int, device) -> int:
     """The chunk's number of sequences, its lengths and starts checked."""
     import torch
@@ -161,7 +186,8 @@ class QueryKeyRotation:
     * ``q_weight``/``k_weight`` ``[D]`` (both BF16 or both float32, either may be
       absent): rows are divided by the root of their mean square plus
       ``norm_eps`` and multiplied by the weight before they turn.
-    * ``q_out``/``k_out``: as ``q``/``k``, which they may be (in place).
+    * ``q_out``/``k_out``: as ``q``/``k``, which they may be (in place); else they
+      share no memory with inputs or each other.
 
     ``prefill(q, k, v, *, first_pos, q_weight=None, k_weight=None) -> (q_stacked,
     kv_current)``: the ``current_len`` tokens at positions ``first_pos ..`` laid
@@ -178,8 +204,8 @@ class QueryKeyRotation:
         self.config = replace(config, backend="hip").validate()
         self.rotary = rotary.validate(self.config.head_dim)
         self.norm_eps = float(norm_eps)
-        if not (math.isfinite(self.norm_eps) and self.norm_eps >= 0):
-            raise ValueError(f"norm_eps must be finite and non-negative, got {norm_eps}")
+        if not (math.isfinite(self.norm_eps) and self.norm_eps >= 2.0**-126):
+            raise ValueError(f"norm_eps must be finite and at least 2^-126, got {norm_eps}")
         self._native = _native
         self._lib = _native.load_library()
         cfg = self.config
@@ -203,8 +229,12 @@ class QueryKeyRotation:
 
     def turns(self, device):
         """Revolutions per position of every pair, float64 on ``device`` (made once per device)."""
+        import torch
+
         got = self._turns.get(device)
         if got is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the first call on a device copies the frequencies there: make it before a capture")
             got = self._turns[device] = (self.rotary.frequencies() / (2 * math.pi)).to(device)
         return got
 
@@ -219,6 +249,8 @@ class QueryKeyRotation:
                     or w.device != device or not w.is_contiguous()):
                 raise ValueError(f"{name} must be contiguous bfloat16 or float32 [{self.config.head_dim}] on {device}, "
                                  f"got {w.dtype} {tuple(w.shape)} on {w.device}")
+            if w.data_ptr() % (4 * w.element_size()):
+                raise ValueError(f"{name} must start at a multiple of {4 * w.element_size()} bytes")
             dtype = w.dtype
         if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
             raise ValueError(f"q_weight and k_weight must share one dtype, got {q_weight.dtype} and {k_weight.dtype}")
@@ -268,6 +300,8 @@ class QueryKeyRotation:
         else:
             _rows("k_out", k_out, cfg.num_kv_heads, cfg.head_dim, n, device)
             _own_places("k_out", k_out)
+        _check_output("q_out", q_out, q, k, k_out)
+        _check_output("k_out", k_out, k, q)
         rotary = self._rotary_args(device, q_weight, k_weight)
         if n == 0:
             return q_out, k_out

@@ -411,16 +411,18 @@ typedef struct pcpa_rotary {
     int32_t interleaved;    /* 0: pairs (i, i + rotary_dim / 2); 1: (2 i, 2 i + 1) */
     int32_t weight_dtype;   /* PCPA_DTYPE_BF16, or PCPA_DTYPE_FP32 */
     float amplitude;        /* finite */
-    float norm_eps;         /* finite, not negative */
+    float norm_eps;         /* finite, at least 2^-126 */
     const double* turns;    /* device [rotary_dim / 2]: revolutions per position */
-    const void* q_weight;   /* device [head_dim], or NULL: Q is not normed */
+    const void* q_weight;   /* device [head_dim], or NULL: Q is not normed; 8-byte (bf16) or 16-byte
+                               (float) aligned */
     const void* k_weight;
 } pcpa_rotary;
 #define PCPA_DTYPE_FP32 3
 
 /*
  * Norms and rotation of the new tokens' Q and K, out of place or in place
- * (q_out / k_out the same rows as q / k).
+ * (q_out / k_out the same rows as q / k; else outputs share no memory with
+ * inputs or each other).
  * Positions, one of: `positions` (device int32 [num_tokens], or int64 with
  * position_bits 64; position_bits 32 otherwise), the chunk's own (positions
  * NULL, position_bits 0), or first_pos + row (position_bits -1; the chunk's
@@ -446,7 +448,8 @@ int32_t pcpa_rotate(const pcpa_params* params, const pcpa_chunk* chunk, const pc
  *                 values that are not finite become NaN codes.  params' k_scale
  *                 and v_scale must be 1.  NULL: as pcpa_kv_cache_write.
  * Rows whose position is negative or beyond the cache, or whose table entry is
- * outside [0, num_pages), are not written.
+ * outside [0, num_pages), are not written.  Of two rows for one place (sequences
+ * that name the same page for new tokens) either may stay, K, V and scales apart.
  */
 int32_t pcpa_chunk_write(const pcpa_params* params, const pcpa_chunk* chunk, const pcpa_rows* k, const pcpa_rows* v,
                          const void* block_table, void* kv_pages, float* token_scales, void* stream);
@@ -475,7 +478,8 @@ int32_t pcpa_cache_read(const pcpa_params* params, int32_t interleave, int64_t f
  * the chunk's K and V already: the row at position p sees positions 0 .. p.
  *   q, out  [num_tokens, num_q_heads, head_dim] bf16
  *   lse     float [num_tokens, num_q_heads] or NULL: as pcpa_history_attention_lse
- * A row that sees nothing (a negative position, no page) gets zeros and -inf.
+ * A row that sees nothing (a negative position, no page) gets zeros and -inf, as
+ * does one whose scores are all -inf.  out may be q, else they share no memory.
  * Both products run on bf16 operands (e4m3 codes widened exactly, the scales
  * applied in 32 bits).  Long walks are cut into ranges when there are few rows;
  * their partials go to `workspace`, device memory of pcpa_chunk_workspace_bytes

@@ -19,7 +19,7 @@ from aws_training_study_amd.pcp_attention import (
     RotaryEmbedding,
     empty_token_scales,
 )
-from aws_training_study_amd.pcp_attention.rotary import _own_places, _rows
+from aws_training_study_amd.pcp_attention.rotary import _check_output, _own_places, _rows, _share_memory
 from chunk_model import FP8, config
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "pcp_attention_hip.h"
@@ -100,6 +100,16 @@ def test_scales_go_with_an_e4m3_pool_and_no_others(lib):
         assert lib.pcpa_cache_read(p, 64, 0, 6, 16, 16, 16, 16, 16, None) == status
 
 
+def test_launches_of_too_many_threads(lib):
+    p = params(head_dim=256, num_q_heads=2, max_local_blocks=1 << 18)
+    c = chunk(batch=1, num_tokens=(1 << 30) - 256)
+    assert lib.pcpa_rotate(p, c, rotary(), 16, 32, 0, rows(), rows(), None, rows(), rows(), None, 0, None) == -8
+    assert lib.pcpa_chunk_write(p, c, rows(), rows(), 16, 16, None, None) == -8
+    assert lib.pcpa_cache_read(p, 64, 0, (1 << 30) - 256, 16, 16, None, 16, 16, None) == -8
+    few = chunk(batch=(1 << 30) - 256, num_tokens=(1 << 30) - 256)
+    assert lib.pcpa_chunk_attention(p, few, 16, 16, None, 16, 16, None, None, 0, None) == -8
+
+
 def test_parameters_are_checked(lib):
     assert lib.pcpa_chunk_attention(params(head_dim=96), chunk(), 16, 16, None, 16, 16, None, None, 0, None) == -5
     assert lib.pcpa_chunk_attention(None, chunk(), 16, 16, None, 16, 16, None, None, 0, None) == -1
@@ -113,7 +123,8 @@ def test_parameters_are_checked(lib):
 @pytest.mark.parametrize("change,status", [
     (dict(rotary_dim=8), -3), (dict(rotary_dim=80), -3), (dict(rotary_dim=-16), -3), (dict(turns=None), -1),
     (dict(turns=20), -6), (dict(amplitude=math.nan), -9), (dict(norm_eps=-1.0), -9), (dict(weight_dtype=2), -4),
-    (dict(q_weight=17), -6), (dict(weight_dtype=3, k_weight=18), -6),
+    (dict(q_weight=17), -6), (dict(weight_dtype=3, k_weight=18), -6), (dict(q_weight=20), -6),
+    (dict(weight_dtype=3, q_weight=24), -6), (dict(norm_eps=0.0), -9), (dict(norm_eps=2.0**-127), -9),
 ])
 def test_rotations_refused(lib, change, status):
     r = rotary(**change)
@@ -173,6 +184,9 @@ def test_embeddings_refused(change, message):
 def test_norm_eps_refused():
     with pytest.raises(ValueError, match="norm_eps"):
         QueryKeyRotation(config(), RotaryEmbedding(64), norm_eps=-1.0)
+    for small in (0.0, 2.0**-127):
+        with pytest.raises(ValueError, match="norm_eps"):
+            QueryKeyRotation(config(), RotaryEmbedding(64), norm_eps=small)
 
 
 def test_frequencies():
@@ -257,3 +271,30 @@ def test_lengths_and_starts():
     for bad in (lengths, torch.zeros(4, dtype=torch.int64), torch.zeros(8, dtype=torch.int32)[::2]):
         with pytest.raises(ValueError, match="chunk_starts must be"):
             _check_lengths(lengths, bad, 3, 6, cpu)
+
+
+def test_shared_memory():
+    """Which rows of two views share memory, against the addresses themselves."""
+    store = torch.zeros(4096, dtype=torch.bfloat16)
+
+    def view(at, n, heads, d, token, head):
+        return torch.as_strided(store, (n, heads, d), (token, head, 1), at)
+
+    def addresses(t):
+        n, heads, d = t.shape
+        return {t.storage_offset() + i * t.stride(0) + h * t.stride(1) + x
+                for i in range(n) for h in range(heads) for x in range(d)}
+
+    views = [view(*v) for v in [(0, 4, 2, 8, 64, 8), (16, 4, 2, 8, 64, 8), (8, 4, 2, 8, 64, 8), (48, 4, 3, 8, 64, 8),
+                                (56, 4, 1, 8, 64, 8), (256, 4, 2, 8, 64, 8), (0, 1, 2, 8, 64, 8), (16, 1, 4, 8, 0, 8),
+                                (1000, 4, 2, 8, 16, 8), (1064, 4, 2, 8, 16, 8), (1024, 4, 2, 8, 16, 8)]]
+    for a in views:
+        for b in views:
+            shared = bool(addresses(a) & addresses(b))
+            assert _share_memory(a, b) or not shared
+            if a.stride(0) == b.stride(0) and a.shape[0] == b.shape[0]:  # (told apart exactly)
+                assert _share_memory(a, b) == shared, (a.storage_offset(), b.storage_offset())
+    _check_output("out", views[0], views[0], views[1])
+    for own, other in ((views[2], views[1]), (views[0], views[2])):
+        with pytest.raises(ValueError, match="out must be its own input"):
+            _check_output("out", views[0], own, other)
