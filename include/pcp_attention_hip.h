@@ -484,6 +484,9 @@ int32_t pcpa_cache_read(const pcpa_params* params, int32_t interleave, int64_t f
  * applied in 32 bits).  Long walks are cut into ranges when there are few rows;
  * their partials go to `workspace`, device memory of pcpa_chunk_workspace_bytes
  * bytes, 16-byte aligned, which needs no initialisation; NULL if that is 0.
+ * pcpa_chunk_workspace_bytes depends on the shapes alone (of `starts` only
+ * whether it is NULL) and returns a status, which is negative, if it refuses
+ * them.  Calls that may overlap need workspaces of their own.
  */
 int64_t pcpa_chunk_workspace_bytes(const pcpa_params* params, const pcpa_chunk* chunk);
 int32_t pcpa_chunk_attention(const pcpa_params* params, const pcpa_chunk* chunk, const void* q, const void* kv_pages,
