@@ -92,6 +92,12 @@ class RotaryEmbedding:
         return freq
 
 
+# Revolutions per position of every pair, for each embedding and device: kept for
+# good, as kernels on any stream and graphs of the caller's own may read them after
+# the object that made them is gone.
+_TURNS = {}
+
+
 def _rows(name: str, t, heads: int, head_dim: int, n: Optional[int], device=None) -> None:
     """``ValueError`` unless ``t`` is ``[n, heads, head_dim]`` BF16 GPU rows the kernels can address."""
     import torch
@@ -194,8 +200,10 @@ class QueryKeyRotation:
     out for ``PrefillAttention``: Q ``[pcp, Hq, local_q, D]`` and K and V ``[2,
     Hkv, current_len, D]`` (whose halves ``KVCacheWriter`` takes).
 
-    Angles are formed in 64 bits and reduced to a turn, the rest is computed in
-    float32 and rounded once.  Asynchronous on the current torch stream.
+    Angles are formed in 64 bits and reduced to a turn (off by less than 2^-22 of
+    one for positions below 2^31), the rest is computed in float32 and rounded
+    once.  Asynchronous on the current torch stream; an embedding's first call on a
+    device copies its frequencies there, which no capture can hold.
     """
 
     def __init__(self, config: PCPAttentionConfig, rotary: RotaryEmbedding, *, norm_eps: float = 1e-6):
@@ -228,14 +236,18 @@ class QueryKeyRotation:
         return call
 
     def turns(self, device):
-        """Revolutions per position of every pair, float64 on ``device`` (made once per device)."""
+        """Revolutions per position of every pair, float64 on ``device`` (made once per embedding and device)."""
         import torch
 
         got = self._turns.get(device)
         if got is None:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the first call on a device copies the frequencies there: make it before a capture")
-            got = self._turns[device] = (self.rotary.frequencies() / (2 * math.pi)).to(device)
+            got = _TURNS.get((self.rotary, device))
+            if got is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("an embedding's first call on a device copies its frequencies there: make one "
+                                       "before a capture")
+                got = _TURNS.setdefault((self.rotary, device), (self.rotary.frequencies() / (2 * math.pi)).to(device))
+            self._turns[device] = got
         return got
 
     def _rotary_args(self, device, q_weight, k_weight):

@@ -109,6 +109,45 @@ def test_attention_into_q(options, lengths, fresh, cuda_device):
                out=both[1:], **scales)
 
 
+# ---- objects that go before their work --------------------------------------------------
+
+
+def test_a_graph_outlives_the_rotation_it_recorded(cuda_device):
+    cfg = config(hq=4, hkv=2, d=64)
+    rotary = RotaryEmbedding(64, base=12345.0)
+    q, k = (rows(torch.Generator().manual_seed(20), 9, h, 64).to(cuda_device) for h in (4, 2))
+    positions = torch.arange(100, 109, dtype=torch.int32, device=cuda_device)
+    want = [x.clone() for x in QueryKeyRotation(cfg, rotary)(q, k, positions=positions)]
+    op = QueryKeyRotation(cfg, rotary)
+    op(q, k, positions=positions)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = op(q, k, positions=positions)
+    del op
+    others = [torch.zeros(32, dtype=torch.float64, device=cuda_device) for _ in range(64)]
+    for _ in range(3):
+        for x in got:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        others[0].add_(1.0)
+
+
+def test_a_first_call_under_capture_is_refused(cuda_device):
+    cfg = config(hq=4, hkv=2, d=64)
+    op = QueryKeyRotation(cfg, RotaryEmbedding(64, base=54321.0))
+    q, k = (rows(torch.Generator().manual_seed(21), 3, h, 64).to(cuda_device) for h in (4, 2))
+    positions = torch.arange(3, dtype=torch.int32, device=cuda_device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="before a capture"):
+            op(q, k, positions=positions)
+        positions.add_(0)
+    op(q, k, positions=positions)
+
+
 # ---- scores --------------------------------------------------------------------------
 
 
