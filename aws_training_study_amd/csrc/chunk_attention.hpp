@@ -35,7 +35,8 @@ struct AttendArgs {
     float* lse;
     int32_t num_q_heads;
     int32_t group;
-    int32_t rows;          // of a workgroup's row tile
+    int32_t rows_log2;     // of a workgroup's row tile
+    Div div_group, div_heads;
     int32_t max_items;     // the launch's workgroups
     int32_t slots;         // workgroups that the GPU holds at once
     int32_t min_range;     // tiles a range has at least
@@ -61,23 +62,34 @@ struct Item {
 // positions, so that with chunks of 64 they follow the positions.  Tile i is
 // local positions 64 (i / pcp) .. of rank i % pcp; a few may be empty.
 __device__ __forceinline__ int walk_tiles(const Pages& p, int keys) {
-    const int most = (int)paging::owned_below(keys, 0, p.pcp, p.interleave);
-    return p.pcp * ((most + kTileKeys - 1) / kTileKeys);
+    return p.pcp * ((owned_of(p, keys, 0) + kTileKeys - 1) / kTileKeys);
+}
+
+// The row of q and out that row `r` of the item's sequence and KV head is.
+__device__ __forceinline__ int64_t row_index(const AttendArgs& a, const Item& it, int r) {
+    const int token = (int)div((uint32_t)r, a.div_group);
+    return (int64_t)(it.span.first + token) * a.num_q_heads + it.head * a.group + (r - token * a.group);
 }
 
 // The place of item `at` among the items of its sequence; false for none.
 __device__ __forceinline__ bool place_item(const AttendArgs& a, int at, int walk, Item& it) {
     const int heads = a.pages.num_kv_heads;
     if (at < 0) return false;
-    const int rest = at / heads;
+    const int rest = (int)div((uint32_t)at, a.div_heads);
     it.head = at - rest * heads;
-    it.range = rest / it.plan.tiles;
+    it.range = it.plan.tiles == 1 ? rest : rest / it.plan.tiles;
     // the last rows, which see the most, first
     it.tile = it.plan.tiles - 1 - (rest - it.range * it.plan.tiles);
     // (starts that decrease may overflow the sums: no such item)
     if (it.range >= it.plan.ranges) return false;
-    it.begin = (int)((int64_t)walk * it.range / it.plan.ranges);
-    it.end = (int)((int64_t)walk * (it.range + 1) / it.plan.ranges);
+    // (the first ranges a tile longer than the rest, if they are not equal)
+    it.begin = 0;
+    it.end = walk;
+    if (it.plan.ranges > 1) {
+        const int whole = walk / it.plan.ranges, more = walk - whole * it.plan.ranges;
+        it.begin = it.range * whole + min(it.range, more);
+        it.end = it.begin + whole + (it.range < more);
+    }
     return true;
 }
 
@@ -93,7 +105,7 @@ __device__ __forceinline__ bool place_item(const AttendArgs& a, int at, int walk
 __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int rows_per_tile, Item& it) {
     const int lane = threadIdx.x & 63, heads = a.pages.num_kv_heads, batch = a.chunk.batch;
     const bool cut = a.part_o != nullptr;
-    auto tiles_of = [&](int count) { return (int)(((int64_t)count * a.group + rows_per_tile - 1) / rows_per_tile); };
+    auto tiles_of = [&](int count) { return (int)(((uint32_t)(count * a.group) + rows_per_tile - 1) / rows_per_tile); };
     // (a sequence whose rows see nothing still has an item, for their zeros)
     auto walk_of = [&](int length) { return max(walk_tiles(a.pages, min(max(length, 0), a.pages.capacity)), 1); };
     if (!cut && !a.chunk.starts) {
@@ -137,8 +149,9 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
         // of 512 to 8192 tokens, 2 heads at D 256, e4m3: 83.2 -> 74.6 us.)
         if (over_all([](int t, int) { return (float)t; }) < slots)
             for (int tries = 0; tries < 6; ++tries) {
-                const int len = (int)length_of;
-                const float count = over_all([&](int t, int w) { return (float)(t * ((w + len - 1) / len)); });
+                // (2^-10: no more than w / length_of where that is a whole number)
+                const float inv = 1.f / length_of;
+                const float count = over_all([&](int t, int w) { return (float)t * ceilf(fmaf((float)w, inv, -0x1p-10f)); });
                 if (count <= slots) break;
                 length_of = fminf(ceilf(fmaxf(length_of + 1.f, length_of * (count / slots))), 0x1p30f);
             }
@@ -292,17 +305,17 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     // the tile's last row sees the most
     const int last = min(row0 + S::ROWS, rows) - 1;
     auto sees = [&](int row) {
-        const int64_t np = (int64_t)it.length - it.span.count + row / a.group + 1;
+        const int64_t np = (int64_t)it.length - it.span.count + (int)div((uint32_t)row, a.div_group) + 1;
         return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
     };
+    auto index_of = [&](int row) { return row_index(a, it, row); };
     const int most = __builtin_amdgcn_readfirstlane(sees(last)), least = __builtin_amdgcn_readfirstlane(sees(row0));
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int row = row0 + 16 * rt + r16;
         const bool ok = row < rows;
         seen[rt] = ok ? sees(row) : most;  // rows past the last mask nothing
-        const int tok = it.span.first + row / a.group, hd = it.head * a.group + row % a.group;
-        const uint8_t* const qrow = a.q + ((int64_t)tok * a.num_q_heads + hd) * D * 2;
+        const uint8_t* const qrow = a.q + index_of(row) * D * 2;
 #pragma unroll
         for (int c = 0; c < QK; ++c) {
             const int d = FP8 ? 64 * (c >> 1) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
@@ -313,14 +326,16 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     }
     // striping: whole rounds and the rest of what each row sees
     const int stride = a.pages.pcp * a.pages.interleave;
-    int rounds[RT], rest[RT];
+    auto striped = [&](int keys, int& whole, int& tail) {
+        const int round = (int)div((uint32_t)keys, a.pages.div_stride);
+        whole = round * a.pages.interleave;
+        tail = keys - round * stride;
+    };
+    int rounds[RT], rest[RT], most_rounds, most_rest, least_rounds, least_rest;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        rounds[rt] = seen[rt] / stride * a.pages.interleave;
-        rest[rt] = seen[rt] % stride;
-    }
-    const int most_rounds = most / stride * a.pages.interleave, most_rest = most % stride;
-    const int least_rounds = least / stride * a.pages.interleave, least_rest = least % stride;
+    for (int rt = 0; rt < RT; ++rt) striped(seen[rt], rounds[rt], rest[rt]);
+    striped(most, most_rounds, most_rest);
+    striped(least, least_rounds, least_rest);
     auto owned = [&](int whole, int tail, int rank) {
         return whole + min(max(tail - rank * a.pages.interleave, 0), a.pages.interleave);
     };
@@ -671,8 +686,7 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
                 *(v4f*)(a.part_o + prow * D + 4 * c) = empty ? v4f{0.f, 0.f, 0.f, 0.f} : acc * inv;
                 if (c == 0) a.part_ml[prow] = v2f{top, total};
             } else {
-                const int tok = it.span.first + row / a.group, hd = it.head * a.group + row % a.group;
-                const int64_t at = (int64_t)tok * a.num_q_heads + hd;
+                const int64_t at = index_of(row);
                 uint32_t w[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -737,12 +751,10 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     // (rows past the last do as the last, unseen)
     const int row_c = min(row0 + pw * kRowsPerWave + j, rows - 1);
     auto sees = [&](int r) {
-        const int64_t np = (int64_t)it.length - it.span.count + r / a.group + 1;
+        const int64_t np = (int64_t)it.length - it.span.count + (int)div((uint32_t)r, a.div_group) + 1;
         return (int)min(max(np, (int64_t)0), (int64_t)a.pages.capacity);
     };
-    auto index_of = [&](int r) {
-        return (int64_t)(it.span.first + r / a.group) * a.num_q_heads + it.head * a.group + r % a.group;
-    };
+    auto index_of = [&](int r) { return row_index(a, it, r); };
     const int seen = sees(row_c);
     const int most = __builtin_amdgcn_readfirstlane(sees(min(row0 + kRowsPerGroup, rows) - 1));
     const int least = __builtin_amdgcn_readfirstlane(sees(row0));
@@ -997,12 +1009,11 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     const float inv = empty ? 0.f : z.v_scale / total;
     const float log2sum = empty ? -INFINITY : st.m + __builtin_amdgcn_logf(total);
     if (row >= rows) return;
-    const int64_t row_index =
-        (int64_t)(it.span.first + row / z.group) * z.num_q_heads + it.head * z.group + row % z.group;
+    const int64_t out_row = row_index(z, it, row);
     const bool part = it.plan.ranges > 1;
     const int64_t prow = (int64_t)blockIdx.x * kRowsPerGroup + pw * kRowsPerWave + (lane2 & 31);
     float* const po = z.part_o + prow * D;
-    uint8_t* const orow = z.out + row_index * D * 2;
+    uint8_t* const orow = z.out + out_row * D * 2;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1028,7 +1039,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
         if (part)
             z.part_ml[prow] = v2f{st.m, total};
         else if (z.lse)
-            z.lse[row_index] = log2sum * kLn2;
+            z.lse[out_row] = log2sum * kLn2;
     }
 }
 
@@ -1046,9 +1057,9 @@ __device__ __forceinline__ bool partials_of(const AttendArgs& a, int b, int toke
     const SequencePlan plan = a.plans[b];
     if (plan.ranges <= 1) return false;
     const Span span = span_of(a.chunk, b);
-    const int kv = head / a.group;
+    const int kv = (int)div((uint32_t)head, a.div_group);
     const int row = (token - span.first) * a.group + (head - kv * a.group);
-    const int tile = row / a.rows;
+    const int tile = row >> a.rows_log2;
     const int64_t heads = a.pages.num_kv_heads, item = plan.first_item + ((int64_t)plan.tiles - 1 - tile) * heads + kv;
     const int64_t step = plan.tiles * heads;
     // (only with starts that decrease is there a plan that no workgroup wrote:
@@ -1056,7 +1067,7 @@ __device__ __forceinline__ bool partials_of(const AttendArgs& a, int b, int toke
     if (plan.first_item < 0 || tile >= plan.tiles || step > a.max_items || plan.ranges > a.max_items ||
         item + (plan.ranges - 1) * step >= a.max_items)
         return false;
-    p = Partials{item * a.rows + row % a.rows, step * a.rows, plan.ranges};
+    p = Partials{(item << a.rows_log2) + row - (tile << a.rows_log2), step << a.rows_log2, plan.ranges};
     return true;
 }
 

@@ -9,12 +9,27 @@
 namespace pcpa {
 namespace chunk {
 
+// floor(n / d) for 0 <= n < 2^31 in three instructions: m = floor(2^(31 + l) / d)
+// + 1 with 2^l >= d fits 32 bits and is off from 2^(31 + l) / d by at most one,
+// which n < 2^31 does not carry over a whole number.
+struct Div {
+    uint32_t m;
+    uint32_t shift;
+};
+inline Div make_div(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return Div{(uint32_t)((1ull << (31 + l)) / d + 1), 31 + l};
+}
+__device__ __forceinline__ uint32_t div(uint32_t n, const Div& d) { return (uint32_t)(((uint64_t)n * d.m) >> d.shift); }
+
 struct Desc {
     const int32_t* lengths;  // [batch]
     const int32_t* starts;   // [batch + 1], or null: `each` rows per sequence
     int32_t batch;
     int32_t num_tokens;
     int32_t each;
+    Div div_each;
 };
 
 // The rows [first, first + count) of sequence b, within [0, num_tokens)
@@ -34,7 +49,7 @@ __device__ __forceinline__ Span span_of(const Desc& c, int b) {
 // before the row, 64 at a time: a binary search is six dependent loads for 64
 // sequences, this is one.
 __device__ __forceinline__ int sequence_of(const Desc& c, int token) {
-    if (!c.starts) return token / c.each;
+    if (!c.starts) return (int)div((uint32_t)token, c.div_each);
     const int lane = threadIdx.x & 63;
     int b = 0;
     for (int base = 0; base < c.batch; base += 64) {
@@ -45,20 +60,6 @@ __device__ __forceinline__ int sequence_of(const Desc& c, int token) {
     const Span s = span_of(c, b);
     return token >= s.first && token < s.first + s.count ? b : -1;
 }
-
-// floor(n / d) for 0 <= n < 2^31 in three instructions: m = floor(2^(31 + l) / d)
-// + 1 with 2^l >= d fits 32 bits and is off from 2^(31 + l) / d by at most one,
-// which n < 2^31 does not carry over a whole number.
-struct Div {
-    uint32_t m;
-    uint32_t shift;
-};
-inline Div make_div(uint32_t d) {
-    uint32_t l = 0;
-    while ((1ull << l) < d) ++l;
-    return Div{(uint32_t)((1ull << (31 + l)) / d + 1), 31 + l};
-}
-__device__ __forceinline__ uint32_t div(uint32_t n, const Div& d) { return (uint32_t)(((uint64_t)n * d.m) >> d.shift); }
 
 // Over the 64 lanes, by DPP within 16 lanes and by row and half swaps beyond
 // (the shuffles go through LDS, ten times the wait).  f has to be commutative;

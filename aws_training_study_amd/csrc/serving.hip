@@ -42,7 +42,8 @@ int32_t check_pages(const pcpa_params* p, const void* block_table, const void* k
 }
 
 Desc desc_of(const pcpa_chunk* c) {
-    return Desc{c->lengths, c->starts, c->batch, c->num_tokens, c->starts ? 0 : c->num_tokens / c->batch};
+    const int32_t each = c->starts ? 0 : c->num_tokens / c->batch;
+    return Desc{c->lengths, c->starts, c->batch, c->num_tokens, each, make_div(each > 0 ? (uint32_t)each : 1u)};
 }
 
 Pages pages_of(const pcpa_params* p, int32_t interleave, const void* block_table) {
@@ -276,7 +277,9 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     a.lse = lse;
     a.num_q_heads = p->num_q_heads;
     a.group = p->num_q_heads / p->num_kv_heads;
-    a.rows = w.kernel.rows;
+    a.rows_log2 = __builtin_ctz(w.kernel.rows);
+    a.div_group = make_div((uint32_t)a.group);
+    a.div_heads = make_div((uint32_t)p->num_kv_heads);
     a.max_items = (int32_t)w.items;
     a.slots = kCUs * w.kernel.per_cu;
     a.min_range = w.kernel.min_range;

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(TokenArgs a) {
             Span s{0, 0};
             int64_t length = 0;
             if (!a.chunk.starts) {
-                b = token / a.chunk.each;
+                b = (int)div((uint32_t)token, a.chunk.div_each);
                 s = span_of(a.chunk, b);
                 length = a.chunk.lengths[b];
             } else if (a.chunk.batch <= 64) {
