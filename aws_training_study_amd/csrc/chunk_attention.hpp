@@ -40,6 +40,7 @@ struct AttendArgs {
     int32_t max_items;     // the launch's workgroups
     int32_t slots;         // workgroups that the GPU holds at once
     int32_t min_range;     // tiles a range has at least
+    int32_t whole;         // tiles of a walk that is not cut
     float score_scale;     // softmax_scale * k_scale * log2(e)
     float v_scale;
     float* part_o;         // [max_items, rows, D] fp32 normalised outputs of ranges
@@ -151,7 +152,9 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
             for (int tries = 0; tries < 6; ++tries) {
                 // (2^-10: no more than w / length_of where that is a whole number)
                 const float inv = 1.f / length_of;
-                const float count = over_all([&](int t, int w) { return (float)t * ceilf(fmaf((float)w, inv, -0x1p-10f)); });
+                const float count = over_all([&](int t, int w) {
+                    return (float)t * (w <= a.whole ? 1.f : ceilf(fmaf((float)w, inv, -0x1p-10f)));
+                });
                 if (count <= slots) break;
                 length_of = fminf(ceilf(fmaxf(length_of + 1.f, length_of * (count / slots))), 0x1p30f);
             }
@@ -160,7 +163,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
     int before = 0;
     bool found = false;
     auto look = [&](int base, const Lane& x, int t, int w) {
-        const int ranges = (w + range - 1) / range, items = t * heads * ranges, incl = inclusive_sum(items);
+        const int ranges = w <= a.whole ? 1 : (w + range - 1) / range, items = t * heads * ranges, incl = inclusive_sum(items);
         const uint64_t past = __builtin_amdgcn_ballot_w64(before + incl > index);
         if (past) {
             const int src = __builtin_ctzll(past);
@@ -250,6 +253,7 @@ struct FewShape {
     static constexpr int LDS = V_LDS > O_LDS ? V_LDS : O_LDS;
     static constexpr int PER_CU = FP8 && !(D == 256 && RT == 2) ? 2 : 1;  // workgroups that fit
     static constexpr int ROWS = 16 * RT;
+    static constexpr int WHOLE = ROW > 256 ? 4 : 8;  // tiles of a walk that is not cut
 };
 
 // Chunk swizzle of V's rows in LDS.  A transposing read of 8-bit values takes

@@ -181,12 +181,17 @@ int32_t write_chunk(const pcpa_params* p, const pcpa_chunk* c, const pcpa_rotary
 
 // A range of a walk has at least this many tiles (64 keys each).  Few rows: one
 // token over 1024 to 8192 keys at D 256 took 16.4 us a call with 8, 14.5 with 4,
-// 12.6 to 13.9 with 2; many: a range's start costs several tiles' time.
+// 12.6 to 13.9 with 2; many: a range's start costs several tiles' time.  Short
+// walks of few rows stay whole: 32 sequences of 512 tokens, 16 over 2 heads, took
+// 8.6 us where ranges of two tiles took 10.9 (bf16 at D 64), 9.5 and 12.3 (e4m3 at
+// D 128), 13.1 and 17.5 (e4m3 at D 256); one such sequence alone 8.2 and 9.1, 8.5
+// and 9.1, 11.2 and 10.1, and at D 256 bf16 15.6 and 11.3, where 4 tiles are the
+// most.
 constexpr int kMinRangeFew = 2, kMinRangeMany = 8;
 
 struct AttendKernel {
     const void* fn;
-    int threads, rows, per_cu, min_range;
+    int threads, rows, per_cu, min_range, whole;
 };
 // (a kernel with and without token scales has the same shape)
 template <int D, bool FP8, int RT>
@@ -194,7 +199,7 @@ AttendKernel few_kernel(bool scaled) {
     using S = FewShape<D, FP8, RT>;
     return AttendKernel{scaled ? (const void*)attend_few_kernel<D, FP8, FP8, RT>
                                : (const void*)attend_few_kernel<D, FP8, false, RT>,
-                        S::THREADS, S::ROWS, S::PER_CU, kMinRangeFew};
+                        S::THREADS, S::ROWS, S::PER_CU, kMinRangeFew, S::WHOLE};
 }
 template <bool FP8, int RT>
 AttendKernel few_kernel_for(int d, bool scaled) {
@@ -208,7 +213,7 @@ AttendKernel many_kernel(bool scaled) {
     using S = TileShape<D, FP8, false>;
     return AttendKernel{scaled ? (const void*)attend_many_kernel<D, FP8, FP8>
                                : (const void*)attend_many_kernel<D, FP8, false>,
-                        S::THREADS, kRowsPerGroup, S::PAIR ? 1 : 2, kMinRangeMany};
+                        S::THREADS, kRowsPerGroup, S::PAIR ? 1 : 2, kMinRangeMany, kMinRangeMany};
 }
 template <bool FP8>
 AttendKernel many_kernel_for(int d, bool scaled) {
@@ -236,7 +241,8 @@ AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = 
     // row tiles of one KV head: at most one that is not full per sequence
     const int64_t tiles = c->num_tokens * group / w.kernel.rows + sequences;
     const int64_t slots = (int64_t)kCUs * w.kernel.per_cu;
-    w.ranges = c->num_tokens > 0 && tiles * p->num_kv_heads < 4 * slots;
+    const int64_t longest = (int64_t)p->pcp_size * p->max_local_blocks * p->block_size / kTileKeys;
+    w.ranges = c->num_tokens > 0 && tiles * p->num_kv_heads < 4 * slots && longest > w.kernel.whole;
     // (the device sums the work in 32-bit floats, which may be less by 2^-24 for each
     // of a lane's sequences)
     w.items = tiles * p->num_kv_heads + (w.ranges ? slots + slots / 64 : 0);
@@ -283,6 +289,7 @@ int32_t attend(const pcpa_params* p, const pcpa_chunk* c, const void* q, const v
     a.max_items = (int32_t)w.items;
     a.slots = kCUs * w.kernel.per_cu;
     a.min_range = w.kernel.min_range;
+    a.whole = w.kernel.whole;
     a.score_scale = p->softmax_scale * p->k_scale * kLog2e;
     a.v_scale = p->v_scale;
     if (w.ranges) {
