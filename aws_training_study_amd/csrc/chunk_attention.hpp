@@ -98,11 +98,13 @@ __device__ __forceinline__ bool place_item(const AttendArgs& a, int at, int walk
 // workgroup finds it by itself (a launch of its own for this took longer), a
 // sequence to a lane: first the work of the whole chunk, which gives the tiles a
 // range should have so that all ranges fill the GPU once, then the sequence that
-// the index falls into.  The first 64 sequences stay in registers (as many as
-// 256, with their loads in flight together, took more of the registers than they
-// saved: seven prompts, D 256, e4m3: 672 -> 702 us).  Sequences of as many rows
-// each whose walks are not cut need no sums (4096 workgroups of one tile each:
-// 300 -> 268 us).
+// the index falls into.  The first 64 KEPT sequences stay in registers, their
+// loads in flight together: 256 where there are few rows and more sequences than
+// 64 (200 sequences of up to 256 tokens: 17.2 -> 14.4 us; 64 of them 7.9 -> 9.2),
+// else 64 (with many rows the registers have other uses: seven prompts, D 256,
+// e4m3: 672 -> 702 us with 256).  Sequences of as many rows each whose walks are not cut need no
+// sums (4096 workgroups of one tile each: 300 -> 268 us).
+template <int KEPT>
 __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int rows_per_tile, Item& it) {
     const int lane = threadIdx.x & 63, heads = a.pages.num_kv_heads, batch = a.chunk.batch;
     const bool cut = a.part_o != nullptr;
@@ -127,34 +129,52 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
         if (base + lane < batch) x = Lane{span_of(a.chunk, base + lane), a.chunk.lengths[base + lane]};
         return x;
     };
-    const Lane kept = load(0);
-    const int tiles = tiles_of(kept.span.count), walk = walk_of(kept.length);
+    Lane kept[KEPT];
+    int tiles[KEPT], walk[KEPT];
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+        kept[k] = Lane{{0, 0}, 0};
+        if (64 * k < batch) kept[k] = load(64 * k);
+    }
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k) {
+        tiles[k] = tiles_of(kept[k].span.count);
+        walk[k] = walk_of(kept[k].length);
+    }
     int range = 1 << 30;  // (beyond any walk)
     if (cut) {
-        // f(tiles, walk) summed over the sequences (in 32-bit floats: only the
-        // range's length comes of them)
+        // f(tiles, walk) of every sequence
         auto over_all = [&](auto f) {
-            float sum = f(tiles, walk);
-            for (int base = 64; base < batch; base += 64) {
+#pragma unroll
+            for (int k = 0; k < KEPT; ++k)
+                if (64 * k < batch) f(tiles[k], walk[k]);
+            for (int base = 64 * KEPT; base < batch; base += 64) {
                 const Lane x = load(base);
-                sum += f(tiles_of(x.span.count), walk_of(x.length));
+                f(tiles_of(x.span.count), walk_of(x.length));
             }
-            return sum_over_lanes<64>(sum) * heads;
         };
+        // (sums in 32-bit floats: only the range's length comes of them)
         const float slots = (float)a.slots;
-        const float share = ceilf(over_all([](int t, int w) { return (float)t * (float)w; }) / slots);
+        float work = 0.f, least = 0.f;
+        over_all([&](int t, int w) {
+            work += (float)t * (float)w;
+            least += (float)t;
+        });
+        const float share = ceilf(sum_over_lanes<64>(work) * heads / slots);
         float length_of = fmaxf(fminf(share, 0x1p30f), (float)a.min_range);
         // Each sequence's last range is a shorter one, so that ranges of the fair
         // share are more than the GPU holds at once, and the few left over would run
         // after all others: longer ranges, until all run together.  (64 sequences
         // of 512 to 8192 tokens, 2 heads at D 256, e4m3: 83.2 -> 74.6 us.)
-        if (over_all([](int t, int) { return (float)t; }) < slots)
+        if (sum_over_lanes<64>(least) * heads < slots)
             for (int tries = 0; tries < 6; ++tries) {
                 // (2^-10: no more than w / length_of where that is a whole number)
                 const float inv = 1.f / length_of;
-                const float count = over_all([&](int t, int w) {
-                    return (float)t * (w <= a.whole ? 1.f : ceilf(fmaf((float)w, inv, -0x1p-10f)));
+                float count = 0.f;
+                over_all([&](int t, int w) {
+                    count += (float)t * (w <= a.whole ? 1.f : ceilf(fmaf((float)w, inv, -0x1p-10f)));
                 });
+                count = sum_over_lanes<64>(count) * heads;
                 if (count <= slots) break;
                 length_of = fminf(ceilf(fmaxf(length_of + 1.f, length_of * (count / slots))), 0x1p30f);
             }
@@ -178,8 +198,10 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, int index, int ro
         before += __builtin_amdgcn_readlane(incl, 63);
         return false;
     };
-    if (look(0, kept, tiles, walk)) return found;
-    for (int base = 64; base < batch; base += 64) {
+#pragma unroll
+    for (int k = 0; k < KEPT; ++k)
+        if (64 * k < batch && look(64 * k, kept[k], tiles[k], walk[k])) return found;
+    for (int base = 64 * KEPT; base < batch; base += 64) {
         const Lane x = load(base);
         if (look(base, x, tiles_of(x.span.count), walk_of(x.length))) return found;
     }
@@ -295,7 +317,8 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
     __shared__ float wave_ml[S::WAVES][16][2];
 
     Item it;
-    if (!find_item(a, blockIdx.x, S::ROWS, it)) return;
+    if (!(a.chunk.batch <= 64 ? find_item<1>(a, blockIdx.x, S::ROWS, it) : find_item<4>(a, blockIdx.x, S::ROWS, it)))
+        return;
     if (it.head == 0 && it.tile == 0 && it.range == 0 && threadIdx.x == 0 && a.plans) a.plans[it.b] = it.plan;
 
     const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -740,7 +763,7 @@ __global__ void __launch_bounds__((TileShape<D, FP8, false>::THREADS), (TileShap
     __shared__ int spoiled;  // a value that is not finite was taken out of some tile's V
 
     Item it;
-    if (!find_item(a, blockIdx.x, kRowsPerGroup, it)) return;
+    if (!find_item<1>(a, blockIdx.x, kRowsPerGroup, it)) return;
     if (threadIdx.x == 0) spoiled = 0;  // (the first tile's barrier comes before any settle_v)
     if (it.head == 0 && it.tile == 0 && it.range == 0 && threadIdx.x == 0 && a.plans) a.plans[it.b] = it.plan;
 
