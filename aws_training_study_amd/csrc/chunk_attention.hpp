@@ -245,7 +245,9 @@ __device__ __forceinline__ int page_of(const Pages& p, const TableEntry& e) {
 //     are keys 8 g + 4 t + i: the B operand of the next product as they stand.
 //   * the running maximum m, sum l and O^T of each row stay in registers; m is
 //     raised only when a step exceeds it by 2^8 (as in the tile kernel).
-//   * O^T += V^T P^T.  V goes into the wave's own LDS by DMA, 16-byte chunks
+//   * O^T += V^T P^T, P as two bf16 values, the upper half of its bits and the rest
+//     (2^-16 off): rounded to one, it was as far off as the rounding of the result
+//     (0.0024 of it instead of 0.0017), and these MFMAs are not what bounds.  V goes into the wave's own LDS by DMA, 16-byte chunks
 //     swizzled by key so that the transposing reads find every bank once.
 // The next step's K (registers) and V (LDS) load while this one is computed: 16
 // KB (e4m3) or 32 KB (bf16) in flight per wave, 128 KB per CU.  The waves' results
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
             }
         }
         // ---- softmax ---------------------------------------------------------------
-        v8bf pop[RT][KG];
+        v8bf pop[RT][KG], low[RT][KG];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int vis = owned(rounds[rt], rest[rt], st.rank) - st.local;
@@ -607,8 +609,12 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
                 for (int i = 0; i < 4; ++i) {
                     const float p = __builtin_amdgcn_exp2f(s[rt][t][i] - m[rt]);
                     l[rt] += p;
-                    // (one rounding: 2^-8 of each probability, of either sign)
-                    pop[rt][t >> 1][4 * (t & 1) + i] = (__bf16)(SCALED ? p * L.vs[t][i] : p);
+                    const float x = SCALED ? p * L.vs[t][i] : p;
+                    const float high = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+                    pop[rt][t >> 1][4 * (t & 1) + i] = (__bf16)high;
+                    // (the 2^-30: where x is its own upper half, the lower is not a 0
+                    // that made infinite values NaN)
+                    low[rt][t >> 1][4 * (t & 1) + i] = (__bf16)fmaf(x, 0x1p-30f, x - high);
                 }
         }
         issue_scales(nxt);
@@ -639,8 +645,10 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
                     constexpr int e = decltype(ec)::value, op = 4 * n + e, dt = op / KG, kg = op % KG;
                     const v8bf vop = __builtin_bit_cast(v8bf, e4m3x8_to_bf16x8(x[n & 1][e][0], x[n & 1][e][1]));
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
+                    for (int rt = 0; rt < RT; ++rt) {
+                        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, low[rt][kg], o[rt][dt], 0, 0, 0);
                         o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rt][kg], o[rt][dt], 0, 0, 0);
+                    }
                 });
             });
         } else {
@@ -664,8 +672,10 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
                     const v4i w{x[n & 1][2 * e][0], x[n & 1][2 * e][1], x[n & 1][2 * e + 1][0], x[n & 1][2 * e + 1][1]};
                     const v8bf vop = __builtin_bit_cast(v8bf, w);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
+                    for (int rt = 0; rt < RT; ++rt) {
+                        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, low[rt][kg], o[rt][dt], 0, 0, 0);
                         o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vop, pop[rt][kg], o[rt][dt], 0, 0, 0);
+                    }
                 });
             });
         }

@@ -42,6 +42,8 @@ WRITES = {
     "uneven": (dict(pcp=3, il=48, block=192, d=64, hkv=8, hq=24, kv=FP8), [500, 145], [45, 145]),
     "striped_bf16": (dict(pcp=5, il=32, block=64, d=256, hkv=1, hq=4), [333, 9], [333, 9]),
     "many_rows": (dict(d=64, hkv=2, hq=8, kv=FP8, bucket=8192), [8000, 5000], [8000, 4900]),
+    "many_sequences": (dict(d=64, hkv=3, hq=6, kv=FP8, bucket=256), [5 + 3 * i % 200 for i in range(150)],
+                       [i % 5 for i in range(150)]),
 }
 
 

@@ -207,6 +207,10 @@ UNEVEN = [
     # more sequences than a wave has lanes, many rows of each
     (dict(d=128, hq=8, hkv=1, bucket=256), [40 + i for i in range(140)], [5 + i % 9 for i in range(140)]),
     (dict(d=256, kv=FP8, hq=16, hkv=2, bucket=256), [40 + i for i in range(70)], [(i % 3) * 4 for i in range(70)]),
+    # more sequences than the registers keep: of few rows, cut into ranges or not, and of many
+    (dict(d=64, hq=2, hkv=1, bucket=1024), [1 + (37 * i) % 90 for i in range(299)] + [1000], [i % 3 for i in range(300)]),
+    (dict(d=64, hq=2, hkv=1, bucket=128), [1 + (37 * i) % 90 for i in range(300)], [1] * 300),
+    (dict(d=64, hq=8, hkv=1, bucket=1024), [20 + (37 * i) % 90 for i in range(299)] + [900], [6] * 300),
     # equal rows of many sequences without ranges
     (dict(d=64, hq=32, hkv=4, bucket=256), [100 + i for i in range(130)], [32] * 130),
 ]
