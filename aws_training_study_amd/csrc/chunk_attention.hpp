@@ -254,7 +254,7 @@ __device__ __forceinline__ int page_of(const Pages& p, const TableEntry& e) {
 // meet in LDS at the end.
 // HBM bound once walks are long: 64 sequences of 4544 tokens, 2 heads at D 256,
 // e4m3 with token scales, 57 us with the merge, 5.2 TB/s (5.5 without scales); of
-// 512 to 8192 tokens 68 us, as the longest range is 21 tiles where 18 would be
+// 512 to 8192 tokens 67 us, as the longest range is 21 tiles where 18 would be
 // equal shares, and a tile of a range is half a step of its four waves.
 template <int D, bool FP8, int RT>
 struct FewShape {
@@ -746,7 +746,8 @@ __global__ void __launch_bounds__((FewShape<D, FP8, RT>::THREADS),
 // widening of K and V beside it: 512 new tokens of 32768, 64 over 8 heads at D 128,
 // bf16, 540 us (1.0 PFLOP/s, where a bf16 matrix product of the library reaches
 // 1.3); seven prompts of up to 4096 tokens, 32 over 2 heads at D 256, e4m3 with
-// token scales, 670 us (0.80).
+// token scales, 665 us (0.80).  P is rounded once to bf16: as two values, as for few
+// rows, the two took 754 and 914 us.
 
 // The sequence's walk for one workgroup: tile i of [begin, end) as find_item
 // counts them.

@@ -231,8 +231,9 @@ class ChunkAttentionKernel(_CacheOperator):
       (device, stream, thread).
 
     Both products run on BF16 operands whatever the cache holds: e4m3 codes are
-    widened exactly, the scales applied in float32.  Asynchronous on the current
-    stream.
+    widened exactly, the scales applied in float32, the probabilities as two BF16
+    values or, where sequences have many rows (over 32 a KV head on average), rounded
+    to one.  Asynchronous on the current stream.
     """
 
     def __init__(self, config: PCPAttentionConfig):
