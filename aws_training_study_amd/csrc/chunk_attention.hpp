@@ -235,7 +235,7 @@ __device__ __forceinline__ int page_of(const Pages& p, const TableEntry& e) {
 // ---- few rows ------------------------------------------------------------------
 //
 // For up to 32 rows per (sequence, KV head) - one token of a GQA group, or a few
-// - the work is reading the cache once: every wave streams its own keys, no wave
+// - or few in all, the work is reading the cache once: every wave streams its own keys, no wave
 // waits for another.  A step of a wave is KEYS keys:
 //   * S^T = K Q^T by 16x16x32 MFMAs.  K goes from the pages straight into the A
 //     operand's registers: lane 16 g + r holds 16 bytes of the key in row r, four

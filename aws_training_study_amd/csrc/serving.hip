@@ -234,7 +234,12 @@ AttendPlan attend_plan(const pcpa_params* p, const pcpa_chunk* c, bool scaled = 
     const bool narrow = sequences > 0 && c->num_tokens * group <= 16 * sequences;
     const bool fp8 = p->kv_dtype == PCPA_DTYPE_FP8_E4M3FN;
     const int d = p->head_dim;
-    const bool many = c->num_tokens * group > 32 * sequences;
+    // Few rows: 32 a sequence and KV head on average, or so few in all that the
+    // kernel for them runs on half of the CUs at most (8 new tokens of each of 8
+    // sequences of 512, 32 over 2 heads at D 256, e4m3: 19.2 us, with the other 26.7;
+    // on all of them, 128 of 128 tokens, 64 over 8 at D 128, bf16: 11.2 and 9.0)
+    const int64_t few_tiles = c->num_tokens * group / 32 + sequences;
+    const bool many = c->num_tokens * group > 32 * sequences && few_tiles * p->num_kv_heads > kCUs / 2;
     w.kernel = many  ? (fp8 ? many_kernel_for<true>(d, scaled) : many_kernel_for<false>(d, false))
                : fp8 ? (narrow ? few_kernel_for<true, 1>(d, scaled) : few_kernel_for<true, 2>(d, scaled))
                      : (narrow ? few_kernel_for<false, 1>(d, false) : few_kernel_for<false, 2>(d, false));

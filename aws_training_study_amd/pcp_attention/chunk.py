@@ -232,8 +232,8 @@ class ChunkAttentionKernel(_CacheOperator):
 
     Both products run on BF16 operands whatever the cache holds: e4m3 codes are
     widened exactly, the scales applied in float32, the probabilities as two BF16
-    values or, where sequences have many rows (over 32 a KV head on average), rounded
-    to one.  Asynchronous on the current stream.
+    values or, where there are many rows (over 32 a sequence and KV head on average
+    and over about 4000 in all), rounded to one.  Asynchronous on the current stream.
     """
 
     def __init__(self, config: PCPAttentionConfig):
