@@ -69,6 +69,13 @@ CASES = {
     # rows enough to fill the GPU several times over (walks are not cut into ranges)
     "many_rows": (dict(d=64, hq=32, hkv=2, bucket=640), [600, 520, 1], [600, 520, 1]),
     "many_rows_fp8": (dict(d=128, kv=FP8, hq=32, hkv=2, bucket=1280), [640, 1280, 3], [500, 620, 1]),
+    # rows enough for the kernel that shares its tiles, with walks that are cut and not
+    "many_d64_long": (dict(d=64, hq=64, hkv=2, block=128, bucket=1280), [1000, 90], [70, 20]),
+    "many_d128_fp8_long": (dict(d=128, kv=FP8, hq=64, hkv=2, bucket=1280), [700], [70]),
+    "many_d128_striped": (dict(pcp=3, il=48, block=192, d=128, hq=64, hkv=2), [300, 0, 200], [70, 0, 31]),
+    "many_d256": (dict(d=256, hq=64, hkv=2, bucket=640), [600, 33], [70, 33]),
+    "many_d256_fp8": (dict(pcp=2, il=32, block=64, d=256, kv=FP8, hq=64, hkv=2, bucket=640), [600, 33], [70, 33]),
+    "many_empty_rows": (dict(d=128, hq=64, hkv=2), [5, 0, 70], [60, 3, 71]),
     # more new tokens than the cache holds (rows that see nothing), empty caches
     "empty_rows": (dict(d=128, hq=8, hkv=2), [5, 0, 0, 130], [9, 3, 0, 131]),
     "empty_rows_fp8": (dict(d=256, kv=FP8, hq=32, hkv=2), [2, 0], [4, 1]),
@@ -123,7 +130,7 @@ def test_no_rows(cuda_device):
 
 
 @pytest.mark.parametrize("dtype,bad", [(torch.int32, [-1, -7, 10**6]), (torch.int64, [-1, 2**32, 2**40 + 1])])
-@pytest.mark.parametrize("fresh", [[1], [90]])
+@pytest.mark.parametrize("fresh", [[1], [90], [600]])
 def test_entries_of_no_page(dtype, bad, fresh, cuda_device):
     """Keys of a table entry that names no page are seen by nobody."""
     cfg = config(pcp=2, il=64, block=64, d=128, hq=8, hkv=2, bucket=1024)
@@ -152,11 +159,11 @@ def test_lengths_beyond_the_cache(cuda_device):
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("d,kv", [(64, BF16), (128, BF16), (256, BF16), (128, FP8), (256, FP8)])
-@pytest.mark.parametrize("fresh", [3, 100])
+@pytest.mark.parametrize("fresh", [3, 100, 300])
 def test_a_later_token_that_is_not_finite(bad, d, kv, fresh, cuda_device):
     """Rows before a token with a K or V that is not finite keep their results."""
     cfg = config(d=d, kv=kv, hq=16, hkv=2, block=128)
-    n = 150
+    n = max(150, fresh + 50)
     gen = torch.Generator().manual_seed(16)
     k, v = rows(gen, n, cfg.num_kv_heads, d), rows(gen, n, cfg.num_kv_heads, d)
     q = rows(gen, fresh, cfg.num_q_heads, d)

@@ -151,37 +151,38 @@ def test_a_first_call_under_capture_is_refused(cuda_device):
 # ---- scores --------------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("d,kv,fresh", [(64, "bfloat16", 1), (256, "bfloat16", 1), (256, "bfloat16", 100),
-                                        (128, "bfloat16", 100), (64, "bfloat16", 5)])
-def test_scores_near_the_types_lowest(d, kv, fresh, cuda_device):
+@pytest.mark.parametrize("d,hq,fresh", [(64, 8, 1), (256, 8, 1), (256, 8, 100), (128, 8, 100), (64, 8, 5),
+                                        (64, 32, 300), (128, 32, 300), (256, 32, 300)])
+def test_scores_near_the_types_lowest(d, hq, fresh, cuda_device):
     """Scores of -2^120: all the same, so that each row is the mean of what it sees.
 
     P is 1 or one power of two, the sums of n of them are exact but for 2^-24 a
     term in the product with V; the result is rounded once."""
-    cfg = config(d=d, kv=kv, hq=8, hkv=2, bucket=512)
+    cfg = config(d=d, hq=hq, hkv=2, bucket=512)
     n = 333
     gen = torch.Generator().manual_seed(7)
     k, v = torch.zeros(n, 2, d, dtype=torch.bfloat16), rows(gen, n, 2, d)
     k[:, :, 0] = -(2.0**62)
     cache = Cache(cfg, [n], 8, tokens=[(k, v)])
-    q = torch.zeros(fresh, 8, d, dtype=torch.bfloat16)
+    q = torch.zeros(fresh, hq, d, dtype=torch.bfloat16)
     q[:, :, 0] = 2.0**62
     out, lse = run(ChunkAttentionKernel(cfg), cache, q, [n], [fresh], cuda_device)
     for i in range(fresh):
         seen = n - fresh + i + 1
-        value = v[:seen].double().repeat_interleave(4, dim=1)
+        value = v[:seen].double().repeat_interleave(hq // 2, dim=1)
         mean, size = value.mean(dim=0), value.abs().mean(dim=0)
         worst = ((out[i].double() - mean).abs() - HALF_STEP * mean.abs() - 2 * seen * 2.0**-24 * size).max().item()
         assert worst <= 2.0**-40, worst
         assert (lse[i].double() / (-(2.0**124) * cfg.softmax_scale) - 1).abs().max().item() <= 2.0**-20
 
 
-def test_scores_of_minus_infinity(cuda_device):
+@pytest.mark.parametrize("hq", [4, 64])
+def test_scores_of_minus_infinity(hq, cuda_device):
     """Rows whose scores are all -inf are zeros, as rows that see nothing; their neighbours are as ever."""
-    cfg = config(d=128, hq=4, hkv=2)
+    cfg = config(d=128, hq=hq, hkv=2)
     lengths, fresh = [90, 70], [2, 70]
     cache = Cache(cfg, lengths, 9)
-    q = rows(torch.Generator().manual_seed(10), 72, 4, 128)
+    q = rows(torch.Generator().manual_seed(10), 72, hq, 128)
     want = run(ChunkAttentionKernel(cfg), cache, q, lengths, fresh, cuda_device)
     k, v = cache.tokens[0]
     k = k.clone()
